@@ -287,9 +287,8 @@ def run(s):
                 "delta": plain_delta}[kind](s)
     import tinystrata_b200 as T
     if kind == "tables":
-        bs, free = s["case"]["block"], s["free_room"][:-1]
-        lens, n_free = T.block_release(s["lens"], s["done"], s["table"], free, s["n_free"], bs)
-        p = T.block_tables(lens, s["new"], s["table"], free, n_free, bs, s["room"])
+        free = s["free_room"][:-1]
+        p = T.block_tables(s["lens"], s["new"], s["table"], free, s["n_free"], s["case"]["block"], s["room"], done=s["done"])
         return dict(lens=p.lens, bounds=p.cu, slots=p.slots, n_free=p.n_free, free=free, table=s["table"])
     if kind == "append":
         T.kv8_append(s["cache"], s["k"], s["v"], s["slots"])
