@@ -31,8 +31,9 @@ _f = C.c_float
 
 def reference_dir() -> str:
     """The TinyStrata source tree the `ref` builds compile from: $REF when set, else a `reference` directory beside
-    this repository (the same rule as oracle/Makefile)."""
-    return os.environ.get("REF") or os.path.abspath(os.path.join(HERE, "..", "..", "reference"))
+    this repository (the same rule as oracle/Makefile).  "" when that directory holds no sources."""
+    tree = os.environ.get("REF") or os.path.abspath(os.path.join(HERE, "..", "..", "reference"))
+    return tree if os.path.isdir(os.path.join(tree, "src")) else ""
 
 
 def build(ref: bool = True) -> None:
