@@ -348,6 +348,93 @@ int tsb_staged_load(const void* host_blobs, void* slots, uint64_t stride, uint64
 int tsb_stage_layer(const int32_t* slot_of, int n_expert, int n_slots, const void* slots, const void* host_blobs,
                     uint64_t stride, void* stage, int whole, void* stream);
 
+/* --------------------------------------------------------------------------------------------- cache of a serving step
+ * What stands around the expert layer in a decode or prompt step: the paged 8-bit key / value cache, its block tables,
+ * attention over it, and the gated delta rule.  Replaces the roles of the reference's INT8 attention and KV cache
+ * (src/qwen35/int8_attention*.cu) and of its Gated DeltaNet chain (src/qwen35/q36_gdn_chain.cuh), with layouts of this
+ * library's own.  Element types by ggml id: F32 = 0, F16 = 1, BF16 = 30.  Strides are in elements; the innermost
+ * dimension is contiguous. */
+
+/* The pools: int8 codes [n_blocks][n_kv_heads][block_size][head_dim] and fp32 scales [n_blocks][n_kv_heads], a value is
+ * code * scale.  block_size 16, 32 or 64; head_dim 64, 128 or 256; code pools 16-byte aligned. */
+typedef struct tsb_kv8 {
+    uint32_t struct_size;   /* sizeof(tsb_kv8) */
+    int32_t n_blocks, block_size, n_kv_heads, head_dim;
+    int8_t *k, *v;
+    float *k_scale, *v_scale;
+} tsb_kv8;
+
+/* One step of the block allocator, in one launch.  lens [n_req]: tokens cached before the step; n_new [n_req]: tokens the
+ * step adds (negative counts as 0); done [n_req] (may be null): non-zero gives the request's ceil(len / block_size)
+ * blocks back, in request order, and leaves it empty (it takes none in this call).  table [n_req][table_stride]: block
+ * ids, the first ceil(len / block_size) of a row valid.  free_list [free_cap] is a stack, free_list[0 .. *n_free).
+ * Blocks given back go on top of it, blocks needed come from its top in request order; a request is served when its
+ * blocks and all earlier requests' are there and its row is wide enough, else it keeps its length and blocks.
+ * Writes lens_out, cu_new [n_req + 1] (prefix sums of n_new, refused requests' tokens included: they are in the caller's
+ * packed rows), slots [cap_tokens] (block * block_size + offset of the step's tokens in packed order; -1 for a refused
+ * request's and past the last), *n_free_out, the new entries of table, and free_list above the old top.  lens_out and
+ * n_free_out must not be lens and n_free.  At most 8192 requests. */
+int tsb_block_tables(const int32_t* lens, const int32_t* n_new, const uint8_t* done, int n_req, int32_t* table,
+                     int64_t table_stride, int table_width, int32_t* free_list, int free_cap, const int32_t* n_free,
+                     int block_size, int32_t* lens_out, int32_t* cu_new, int64_t* slots, int64_t cap_tokens,
+                     int32_t* n_free_out, void* stream);
+
+/* Append n_tok tokens' keys and values ([token][head][head_dim] with the strides given) at slots (as tsb_block_tables
+ * writes them; one outside the cache is skipped).  Tokens of one block follow one another in `slots`, ascending.  Per
+ * (block, head): scale' = max(scale, largest magnitude / 127), the scale counting as 0 when the tokens start the block;
+ * codes already there become rint(code * (scale / scale')), new ones rint(x / scale').  NaN is stored as 0, an infinity
+ * as the largest bf16. */
+int tsb_kv8_append(const tsb_kv8* cache, const void* k, const void* v, int elem_type, int64_t k_tok, int64_t k_head,
+                   int64_t v_tok, int64_t v_head, const int64_t* slots, int64_t n_tok, void* stream);
+/* The cached tokens at slots as values: k, v [n_tok][n_kv_heads][head_dim] of elem_type, 16-byte aligned; zeros for a
+ * slot outside the cache. */
+int tsb_kv8_read(const tsb_kv8* cache, const int64_t* slots, int64_t n_tok, void* k, void* v, int elem_type, void* stream);
+
+typedef struct tsb_kv8_attn {
+    uint32_t struct_size;   /* sizeof(tsb_kv8_attn) */
+    int32_t n_req, q_heads, elem_type;   /* elem_type of q and out */
+    int32_t max_q;          /* at least the longest request's queries */
+    int32_t table_width;    /* valid columns of table */
+    int32_t window;         /* a query sees the last `window` keys up to its own; 0: all of them */
+    float scale;            /* of the scores */
+    int64_t n_tok;          /* rows of q and out */
+    int64_t q_tok, q_head, o_tok, o_head, table_stride;
+} tsb_kv8_attn;
+uint64_t tsb_kv8_attention_workspace_bytes(const tsb_kv8* cache, const tsb_kv8_attn* d);
+/* Causal attention of each request's last queries over its cached keys (the queries' own among them): request r's rows
+ * of q are cu_q[r] .. cu_q[r + 1] (null: max_q rows each), row i of n sits at position lens[r] - n + i and sees the keys
+ * up to its position.  Query head h reads key / value head h / (q_heads / n_kv_heads).  A row without keys is zero.
+ * Scores, maxima, sums and outputs are accumulated in fp32; out has q's type.  A block id outside the cache hides its
+ * keys.  At most 4096 requests.  Workspace 16-byte aligned, its size from the query above (0 when none is needed). */
+int tsb_kv8_attention(const tsb_kv8* cache, const tsb_kv8_attn* d, const void* q, const int32_t* table, const int32_t* lens,
+                      const int32_t* cu_q, void* out, void* workspace, uint64_t ws_bytes, void* stream);
+
+/* --------------------------------------------------------------------------------------------- gated delta rule
+ * Per value head a state S [dim_k][dim_v] (fp32); per token S <- e^g S, u = beta (v - S^T k), S <- S + k u^T,
+ * o = scale S^T q, with q and k first divided by sqrt(sum of squares + eps) when qk_norm.  Value head h reads key head
+ * h / (v_heads / k_heads).  dim_k 64 or 128, dim_v a multiple of 16. */
+typedef struct tsb_delta_desc {
+    uint32_t struct_size;   /* sizeof(tsb_delta_desc) */
+    int32_t elem_type;      /* of q, k, v and o */
+    int32_t n_seq, max_len; /* sequences; at least the longest one's tokens */
+    int32_t k_heads, v_heads, dim_k, dim_v;
+    int32_t n_states;       /* states in state_in / state_out */
+    int32_t qk_norm;
+    float scale, eps;
+    int64_t n_tok;          /* rows of q, k, v, g, beta, o */
+    int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok, o_head;
+    int64_t gb_tok;         /* row stride of g and beta ([token][v_heads]) */
+} tsb_delta_desc;
+/* 0 up to 16 tokens a sequence (the recurrence); else the chunks' tiles. */
+uint64_t tsb_gated_delta_workspace_bytes(const tsb_delta_desc* d);
+/* n_seq sequences through the rule: rows cu_seqlens[b] .. cu_seqlens[b + 1] (null: max_len rows each) from state_in
+ * [n_states][v_heads][dim_k][dim_v], the states after them to state_out (which may be state_in).  state_idx [n_seq]
+ * (null: sequence b has state b) names each sequence's state, no two the same; a negative one starts from zeros and is
+ * not kept.  Up to 16 tokens a sequence run token by token, longer ones in chunks of 64. */
+int tsb_gated_delta(const tsb_delta_desc* d, const void* q, const void* k, const void* v, const float* g, const float* beta,
+                    const float* state_in, float* state_out, const int32_t* state_idx, const int32_t* cu_seqlens, void* o,
+                    void* workspace, uint64_t ws_bytes, void* stream);
+
 /* --------------------------------------------------------------------------------------------- expert parallelism */
 /* Prompt-path experts sharded over the ranks of one node (one process per GPU), dispatch and return over NCCL
  * point-to-point exchanges on NVLink.  The reference runs one GPU per engine; the per-rank body is its prompt branch

@@ -67,6 +67,31 @@ class ExpertLayout(C.Structure):
                 ("bytes", C.c_uint64)]
 
 
+class Kv8(C.Structure):
+    """tsb_kv8: the pools of the paged 8-bit key / value cache."""
+    _fields_ = [("struct_size", C.c_uint32), ("n_blocks", C.c_int32), ("block_size", C.c_int32),
+                ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("k_scale", C.c_void_p), ("v_scale", C.c_void_p)]
+
+
+class Kv8Attn(C.Structure):
+    """tsb_kv8_attn: one attention call over the cache."""
+    _fields_ = [("struct_size", C.c_uint32), ("n_req", C.c_int32), ("q_heads", C.c_int32), ("elem_type", C.c_int32),
+                ("max_q", C.c_int32), ("table_width", C.c_int32), ("window", C.c_int32), ("scale", C.c_float),
+                ("n_tok", C.c_int64), ("q_tok", C.c_int64), ("q_head", C.c_int64), ("o_tok", C.c_int64),
+                ("o_head", C.c_int64), ("table_stride", C.c_int64)]
+
+
+class DeltaRuleDesc(C.Structure):
+    """tsb_delta_desc: one call of the gated delta rule."""
+    _fields_ = [("struct_size", C.c_uint32), ("elem_type", C.c_int32), ("n_seq", C.c_int32), ("max_len", C.c_int32),
+                ("k_heads", C.c_int32), ("v_heads", C.c_int32), ("dim_k", C.c_int32), ("dim_v", C.c_int32),
+                ("n_states", C.c_int32), ("qk_norm", C.c_int32), ("scale", C.c_float), ("eps", C.c_float),
+                ("n_tok", C.c_int64), ("q_tok", C.c_int64), ("q_head", C.c_int64), ("k_tok", C.c_int64),
+                ("k_head", C.c_int64), ("v_tok", C.c_int64), ("v_head", C.c_int64), ("o_tok", C.c_int64),
+                ("o_head", C.c_int64), ("gb_tok", C.c_int64)]
+
+
 _lib = None
 _lock = threading.Lock()
 _p, _i32, _i64, _u64, _f = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64, C.c_float
@@ -147,6 +172,14 @@ SIGNATURES = {
     "tsb_staged_rebalance": (C.c_int, [_p, C.c_int, C.c_int, _p, _p, C.c_int, _p, _p]),
     "tsb_staged_load": (C.c_int, [_p, _p, _u64, _u64, _p, _p, C.c_int, C.c_int, C.c_int, _p]),
     "tsb_stage_layer": (C.c_int, [_p, C.c_int, C.c_int, _p, _p, _u64, _p, C.c_int, _p]),
+    "tsb_block_tables": (C.c_int, [_p, _p, _p, C.c_int, _p, _i64, C.c_int, _p, C.c_int, _p, C.c_int, _p, _p, _p, _i64,
+                                   _p, _p]),
+    "tsb_kv8_append": (C.c_int, [C.POINTER(Kv8), _p, _p, C.c_int, _i64, _i64, _i64, _i64, _p, _i64, _p]),
+    "tsb_kv8_read": (C.c_int, [C.POINTER(Kv8), _p, _i64, _p, _p, C.c_int, _p]),
+    "tsb_kv8_attention_workspace_bytes": (_u64, [C.POINTER(Kv8), C.POINTER(Kv8Attn)]),
+    "tsb_kv8_attention": (C.c_int, [C.POINTER(Kv8), C.POINTER(Kv8Attn), _p, _p, _p, _p, _p, _p, _u64, _p]),
+    "tsb_gated_delta_workspace_bytes": (_u64, [C.POINTER(DeltaRuleDesc)]),
+    "tsb_gated_delta": (C.c_int, [C.POINTER(DeltaRuleDesc), _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _u64, _p]),
 }
 
 
@@ -659,3 +692,5 @@ class DecodeStack:
 
 
 from .layer import MoELayer, StagedExperts  # noqa: E402  (host mirror of the engines' MoE block)
+from .serving import (BlockPlan, KV8Cache, block_tables, gated_delta, kv8_append, kv8_attention,  # noqa: E402
+                      kv8_read)
