@@ -19,6 +19,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <type_traits>
 
 #include "tsb_device.cuh"
 #include "tsb_warp_mma.cuh"
@@ -219,6 +220,11 @@ __device__ __forceinline__ void pow2_scale(float peak, float& up, float& inv) {
     up = __uint_as_float((uint32_t) (268 - e) << 23);
     inv = __uint_as_float((uint32_t) (e - 14) << 23);
 }
+__device__ __forceinline__ float pow2f(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 __device__ __forceinline__ float max4(float a, float b, float c, float d) {
     return fmaxf(fmaxf(fabsf(a), fabsf(b)), fmaxf(fabsf(c), fabsf(d)));
 }
@@ -231,11 +237,21 @@ __device__ __forceinline__ void split_f16(float x0, float x1, uint32_t& hi, uint
     const float2 h = __half22float2(*(const __half2*) &hi);
     lo = pack_f16(x0 - h.x, x1 - h.y);
 }
+// The same of u x0, u x1 (packed fp32 arithmetic).
+__device__ __forceinline__ void split_f16x2(float x0, float x1, float u, uint32_t& hi, uint32_t& lo) {
+    const float2 y = __fmul2_rn(make_float2(x0, x1), make_float2(u, u));
+    hi = pack_f16(y.x, y.y);
+    const float2 h = __half22float2(*(const __half2*) &hi);
+    const float2 d = __ffma2_rn(h, make_float2(-1.0f, -1.0f), y);
+    lo = pack_f16(d.x, d.y);
+}
 template <int E>
-__device__ __forceinline__ float load_t(const void* p, int64_t i) {
-    if constexpr (E == E_F32) return ((const float*) p)[i];
-    else if constexpr (E == E_F16) return __half2float(((const __half*) p)[i]);
-    else return __bfloat162float(((const __nv_bfloat16*) p)[i]);
+using Elem = std::conditional_t<E == E_F32, float, std::conditional_t<E == E_F16, __half, __nv_bfloat16>>;
+template <int E>
+__device__ __forceinline__ void store_t(Elem<E>* p, float v) {
+    if constexpr (E == E_F32) *p = v;
+    else if constexpr (E == E_F16) *p = __float2half_rn(v);
+    else *p = __float2bfloat16_rn(v);
 }
 
 // Chunks before sequence b (every thread of the CTA gets the sum; n_seq is at most a few thousand).
@@ -285,9 +301,10 @@ __device__ __forceinline__ bool find_chunk(const DeltaParams& p, int c, int& b, 
 
 constexpr int LA = 68;   // row pitch (floats) of the triangle and its inverse in shared memory
 
-// X21 = -X22 (A21 X11) for the pairs of S x S blocks along the diagonal, 128 threads: two small fp32 products.
+// In place: A21 <- -X22 (A21 X11) for the pairs of S x S blocks along the diagonal whose blocks X11, X22 are inverses
+// already; 128 threads, two small fp32 products.
 template <int S>
-__device__ __forceinline__ void merge_blocks(const float* A, float* X, float* tmp, int tid) {
+__device__ __forceinline__ void merge_blocks(float* X, float* tmp, int tid) {
     constexpr int RT = S == 32 ? 2 : 1, CT = S == 8 ? 2 : 4;       // a thread's rows and columns of the result
     constexpr int CG = S / CT, LT = S + 4;
     const int per = S * S / (RT * CT), pair = tid / per, in = tid % per;
@@ -295,7 +312,7 @@ __device__ __forceinline__ void merge_blocks(const float* A, float* X, float* tm
     float* T = tmp + pair * S * LT;
 #pragma unroll
     for (int step = 0; step < 2; ++step) {
-        const float* L = step == 0 ? A + (base + S) * LA + base : X + (base + S) * LA + base + S;
+        const float* L = X + (base + S) * LA + base + (step == 0 ? 0 : S);
         const float* B = step == 0 ? X + base * LA + base : T;
         const int ldb = step == 0 ? LA : LT;
         float acc[RT][CT];
@@ -343,18 +360,17 @@ __device__ __forceinline__ void merge_blocks(const float* A, float* X, float* tm
 // three joins of neighbouring blocks: exact arithmetic on the triangle, where powers of A would cancel, with every
 // thread at work (one thread a column over all 64 rows is 2000 dependent steps: 240 us for 8192 tokens, 32 heads).
 template <int E, int DK>
-__global__ void __launch_bounds__(128) k_delta_prepare(const DeltaParams p) {
+__global__ void __launch_bounds__(128, E == E_F32 ? 2 : 4) k_delta_prepare(const DeltaParams p) {
     using T = Tiles<E, DK>;
     constexpr int PL = T::PL, PP = T::PP;
     extern __shared__ __align__(1024) uint8_t sm[];
     uint8_t* kt = sm;                                    // [PL][64][DK]; later M and P planes and the vectors
     uint8_t* qt = sm + PL * T::kTile;
     constexpr int kStageOut = T::kVal > T::kHead ? T::kVal : T::kHead;
-    float* A = (float*) (sm + kStageOut);                // [64][LA]
-    float* X = A + kChunk * LA;                          // [64][LA]
-    float* tmp = X + kChunk * LA;                        // [32][36]
+    float* A = (float*) (sm + kStageOut);                // [64][LA]: the triangle, inverted in place
+    float* tmp = A + kChunk * LA;                        // [32][36]
     __shared__ __align__(16) float rk[kChunk], rq[kChunk], beta[kChunk];
-    __shared__ double gc[kChunk];
+    __shared__ __align__(16) double gc[kChunk];
     __shared__ int sh[8];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int hk = blockIdx.y, rep = p.hv / p.hk;
@@ -390,11 +406,14 @@ __global__ void __launch_bounds__(128) k_delta_prepare(const DeltaParams p) {
                 const int e = e0 + 128 * i, row = e / TPR, piece = e % TPR;
                 float sq = 0.0f, peak = 0.0f;
 #pragma unroll
-                for (int m = 0; m < 8; ++m) sq = fmaf(x[i][m], x[i][m], sq), peak = fmaxf(peak, fabsf(x[i][m]));
+                for (int m = 0; m < 8; ++m) peak = fmaxf(peak, fabsf(x[i][m]));
 #pragma unroll
-                for (int o = TPR / 2; o > 0; o >>= 1) {
-                    sq += __shfl_xor_sync(0xffffffffu, sq, o);
-                    peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+                for (int o = TPR / 2; o > 0; o >>= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+                if (p.norm) {
+#pragma unroll
+                    for (int m = 0; m < 8; ++m) sq = fmaf(x[i][m], x[i][m], sq);
+#pragma unroll
+                    for (int o = TPR / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
                 }
                 float up, inv;
                 pow2_scale(peak, up, inv);
@@ -449,17 +468,23 @@ __global__ void __launch_bounds__(128) k_delta_prepare(const DeltaParams p) {
     const int g = lane >> 2, qd = lane & 3;
     uint8_t* stage = sm;
     float* vec = (float*) (stage + (2 + PP) * T::kSq);
+    // threads 0..63 hold a token's g, 64..127 its beta, one head ahead of their use
+    const int tt = tid & 63;
+    const float* gsrc = (tid < 64 ? p.g : p.beta) + (tok0 + tt) * p.gb_tok + hk * rep;
+    float gnext = tt < live ? gsrc[0] : 0.0f;
     for (int i = 0; i < rep; ++i) {
         const int h = hk * rep + i;
         __syncthreads();                                  // the tiles, or the previous head's planes, are out
-        if (warp == 0) {
+        // e^-200 is 0 in fp32; a sum of -inf would make differences undefined
+        if (tid < 64) gc[tt] = (double) fmaxf(gnext, -200.0f);
+        else beta[tt] = gnext;
+        if (i + 1 < rep && tt < live) gnext = gsrc[i + 1];
+        __syncthreads();
+        if (warp == 0) {                                  // running sums, in units of log 2
             double v[2];
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
-                const int t = w * 32 + lane;
-                // e^-200 is 0 in fp32; a sum of -inf would make differences undefined
-                v[w] = t < live ? (double) fmaxf(p.g[(tok0 + t) * p.gb_tok + h], -200.0f) : 0.0;
-                beta[t] = t < live ? p.beta[(tok0 + t) * p.gb_tok + h] : 0.0f;
+                v[w] = gc[w * 32 + lane] * 1.4426950408889634;
 #pragma unroll
                 for (int o2 = 1; o2 < 32; o2 <<= 1) {
                     const double u = __shfl_up_sync(0xffffffffu, v[w], o2);
@@ -472,34 +497,49 @@ __global__ void __launch_bounds__(128) k_delta_prepare(const DeltaParams p) {
             for (int w = 0; w < 2; ++w) {
                 const int t = w * 32 + lane;
                 gc[t] = v[w];
-                const float e = expf((float) v[w]);
+                const float e = pow2f((float) v[w]);
                 vec[V_EK + t] = e * rk[t];
                 vec[V_EQ + t] = e * rq[t] * p.scale;
-                vec[V_ED + t] = expf((float) (last - v[w])) * rk[t];
-                vec[V_END + t] = expf((float) last);
+                vec[V_ED + t] = pow2f((float) (last - v[w])) * rk[t];
+                vec[V_END + t] = pow2f((float) last);
             }
         }
-        for (int e = tid; e < kChunk * LA / 4; e += 128) ((float4*) X)[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         __syncthreads();
         float pv[8][4], peak[2] = {0.0f, 0.0f};
+        const int row0 = warp * 16 + g;
+        const double gr[2] = {gc[row0], gc[row0 + 8]};
+        const float ar2[2] = {beta[row0] * rk[row0], beta[row0 + 8] * rk[row0 + 8]};
+        const float pr[2] = {rq[row0] * p.scale, rq[row0 + 8] * p.scale};
 #pragma unroll
-        for (int n = 0; n < 8; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = warp * 16 + g + (e >> 1) * 8, c = n * 8 + 2 * qd + (e & 1);
-                const float f = c <= row ? expf((float) (gc[row] - gc[c])) * rk[c] : 0.0f;
-                A[row * LA + c] = c < row ? beta[row] * (rk[row] * (f * kk[n][e])) : 0.0f;
-                pv[n][e] = f * (rq[row] * p.scale * qk[n][e]);
-                peak[e >> 1] = fmaxf(peak[e >> 1], fabsf(pv[n][e]));
+        for (int n = 0; n < 8; ++n) {
+            const int c = n * 8 + 2 * qd;
+            if (n > 2 * warp + 1) {                       // above the diagonal: the joins read zeros there, P is not read
+                *(float2*) (A + row0 * LA + c) = *(float2*) (A + (row0 + 8) * LA + c) = make_float2(0.0f, 0.0f);
+                continue;
             }
+            const double2 gcc = *(const double2*) (gc + c);
+            const float2 rc = *(const float2*) (rk + c);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = row0 + e * 8;
+                const float f0 = c <= row ? pow2f((float) (gr[e] - gcc.x)) * rc.x : 0.0f;
+                const float f1 = c + 1 <= row ? pow2f((float) (gr[e] - gcc.y)) * rc.y : 0.0f;
+                *(float2*) (A + row * LA + c) = make_float2(c < row ? ar2[e] * (f0 * kk[n][2 * e]) : 0.0f,
+                                                            c + 1 < row ? ar2[e] * (f1 * kk[n][2 * e + 1]) : 0.0f);
+                pv[n][2 * e] = f0 * (pr[e] * qk[n][2 * e]);
+                pv[n][2 * e + 1] = f1 * (pr[e] * qk[n][2 * e + 1]);
+                peak[e] = fmaxf(peak[e], fmaxf(fabsf(pv[n][2 * e]), fabsf(pv[n][2 * e + 1])));
+            }
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const int row = warp * 16 + g + e * 8;
+            const int row = row0 + e * 8;
             float up, inv;
             pow2_scale(quad_max(peak[e]), up, inv);
             if (qd == 0) vec[V_FP + row] = inv;
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
+                if (n > 2 * warp + 1) continue;
                 uint32_t hi, lo;
                 split_f16(pv[n][2 * e] * up, pv[n][2 * e + 1] * up, hi, lo);
                 const uint32_t at = swz(row, n, kChunk * 2) + qd * 4;
@@ -508,41 +548,51 @@ __global__ void __launch_bounds__(128) k_delta_prepare(const DeltaParams p) {
             }
         }
         __syncthreads();
-        if (tid < kChunk) {                               // 8 x 8 diagonal blocks
+        if (tid < kChunk) {                               // 8 x 8 diagonal blocks; a block's threads are in one warp
             const int o = tid & ~7, c = tid & 7;
-            float x[8];
+            float x[8], w[8][8];
+#pragma unroll
+            for (int r = 1; r < 8; ++r)
+#pragma unroll
+                for (int m = 0; m < r; ++m) w[r][m] = A[(o + r) * LA + o + m];
+            __syncwarp();
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
                 float a = r == c ? 1.0f : 0.0f;
 #pragma unroll
-                for (int m = 0; m < r; ++m) a = fmaf(-A[(o + r) * LA + o + m], x[m], a);
+                for (int m = 0; m < r; ++m) a = fmaf(-w[r][m], x[m], a);
                 x[r] = a;
-                X[(o + r) * LA + o + c] = a;
+                A[(o + r) * LA + o + c] = a;
             }
         }
         __syncthreads();
-        merge_blocks<8>(A, X, tmp, tid);
-        merge_blocks<16>(A, X, tmp, tid);
-        merge_blocks<32>(A, X, tmp, tid);
+        merge_blocks<8>(A, tmp, tid);
+        merge_blocks<16>(A, tmp, tid);
+        merge_blocks<32>(A, tmp, tid);
         {
-            const int row = tid >> 1, c0 = (tid & 1) * 32;
-            float m[32], top = 0.0f;
+            const int row = tid >> 1, c0 = (tid & 1) * 8;  // pieces c0, c0 + 16, ... up to the row's diagonal tile
+            float m[4][8], top = 0.0f;
 #pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-                const float4 x = *(const float4*) (X + row * LA + c0 + c), w = *(const float4*) (beta + c0 + c);
-                m[c] = x.x * w.x, m[c + 1] = x.y * w.y, m[c + 2] = x.z * w.z, m[c + 3] = x.w * w.w;
-                top = fmaxf(top, max4(m[c], m[c + 1], m[c + 2], m[c + 3]));
+            for (int t = 0; t < 4; ++t) {
+                if (16 * t > row) break;
+#pragma unroll
+                for (int c = 0; c < 8; c += 4) {
+                    const float4 x = *(const float4*) (A + row * LA + 16 * t + c0 + c), w = *(const float4*) (beta + 16 * t + c0 + c);
+                    m[t][c] = x.x * w.x, m[t][c + 1] = x.y * w.y, m[t][c + 2] = x.z * w.z, m[t][c + 3] = x.w * w.w;
+                    top = fmaxf(top, max4(m[t][c], m[t][c + 1], m[t][c + 2], m[t][c + 3]));
+                }
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             float up, inv;
             pow2_scale(top, up, inv);
             if (c0 == 0) vec[V_FM + row] = inv;
 #pragma unroll
-            for (int c = 0; c < 32; c += 8) {
+            for (int t = 0; t < 4; ++t) {
+                if (16 * t > row) break;
                 uint32_t hi[4], lo[4];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) split_f16(m[c + 2 * u] * up, m[c + 2 * u + 1] * up, hi[u], lo[u]);
-                const uint32_t at = swz(row, (c0 + c) >> 3, kChunk * 2);
+                for (int u = 0; u < 4; ++u) split_f16(m[t][2 * u] * up, m[t][2 * u + 1] * up, hi[u], lo[u]);
+                const uint32_t at = swz(row, (16 * t + c0) >> 3, kChunk * 2);
                 *(uint4*) (stage + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                 *(uint4*) (stage + T::kSq + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
@@ -553,17 +603,39 @@ __global__ void __launch_bounds__(128) k_delta_prepare(const DeltaParams p) {
     }
 }
 
-// Two warps that share 16 value columns.
-__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+// The W warps that share 16 value columns.
+template <int W>
+__device__ __forceinline__ void unit_sync(int unit) {
+    if constexpr (W > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + unit), "n"(32 * W) : "memory");
+}
+
+// The power-of-two scales of a left operand's rows g and g + 8, and their inverses: largest magnitudes in [2^9, 2^10), so
+// that the next chunk's may grow 32-fold.
+struct RowScale {
+    float u[2] = {0.0f, 0.0f}, i[2] = {0.0f, 0.0f};
+    __device__ __forceinline__ void set(float a, float c) {
+        pow2_scale(a, u[0], i[0]);
+        pow2_scale(c, u[1], i[1]);
+        u[0] *= 0.03125f, u[1] *= 0.03125f, i[0] *= 32.0f, i[1] *= 32.0f;
+    }
+    // Whether rows with these largest magnitudes fit fp16 pairs under the scales at full accuracy: at most 2^15, and not
+    // so small that the low halves (multiples of 2^-24) lose bits.
+    __device__ __forceinline__ bool holds(float a, float c) const {
+        const float x = a * u[0], y = c * u[1];
+        return x <= 32768.0f && y <= 32768.0f && (x >= 0.25f || a == 0.0f) && (y >= 0.25f || c == 0.0f);
+    }
+};
 
 // CTA (value columns, value head, sequence).  A unit is 16 value columns, held by W warps: S^T [16][DK] stays in their
 // registers in accumulator layout, which is the left operand's layout, and a chunk is five chained products
 //   Y^T = S^T K^T, Z^T = S^T Q^T, U^T = (V^T - e^gc Y^T) M^T, O^T = e^gc Z^T + U^T P^T, S^T = e^gc_63 S^T + U'^T K
 // whose right operands are the chunk's tiles (bulk copies, two chunks deep).  W 1: a warp owns its unit and exchanges
-// nothing, eight units a CTA; W 2: two warps take half of every product's columns (tokens, keys) each and pass the left
-// operands through shared memory, two units a CTA.  What bounds it: a sequence's chunks follow one another, and a unit's
-// 400 products of 16 x 8 x 16 a chunk (bf16, dim_k 128) at 8 cycles each.  One sequence of 32 heads has 256 units, so W 2
-// puts them on 128 SMs with every scheduler at work; with more sequences W 1 does the same work without exchanges.
+// nothing, eight units a CTA; W 2: the warps take half of every product's columns (tokens, keys) each and pass the left
+// operands through shared memory, two units a CTA; operands are written under the scales of the chunk before, and again
+// in the rare case that a row outgrew them, so that an exchange is one barrier.  What bounds it: a sequence's chunks
+// follow one another, and a unit's 400 products of 16 x 8 x 16 a chunk (bf16, dim_k 128) at 8 cycles each.  One sequence
+// of 32 heads has 256 units, so W 2 puts them on 128 SMs with every scheduler at work; with more sequences W 1 does the
+// same work without exchanges.
 template <int E, int DK, int W>
 __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaParams p) {
     using T = Tiles<E, DK>;
@@ -571,11 +643,13 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaPa
     constexpr bool OS = T::PP == 2;
     constexpr int UN = W == 1 ? 8 : 2;                 // units of a CTA
     constexpr int NK = DK / 8 / W, NP = 4 / W;         // a warp's key tiles of 8, token tiles of 16
-    constexpr int kFrag = W == 1 ? 0 : DK / 16 * 2 * 512 + 4 * 2 * 512;   // a unit's exchanged left operands
+    constexpr int NS = NK / 2 < 2 ? NK / 2 : 2;
+    constexpr int kFrag = W == 1 ? 0 : 12 * 1024;      // a unit's exchanged left operands
+    constexpr int RB = DK * 2, SB = kChunk * 2;        // row bytes of the key and of the square tiles
     extern __shared__ __align__(1024) uint8_t sm[];
     __shared__ uint64_t full[2], empty[2];
     __shared__ int sh[8];
-    __shared__ float peaks[UN][2][W][2][16];
+    __shared__ float peaks[UN][4][W][16];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, qd = lane & 3;
     const int unit = warp / W, part = warp % W;
     const int h = blockIdx.y, b = blockIdx.z, hk = h / (p.hv / p.hk);
@@ -586,8 +660,9 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaPa
     const int chunks = min((s.n + kChunk - 1) / kChunk, max(p.max_chunks - first, 0));
     const int n0 = (blockIdx.x * UN + unit) * 16;
     const bool in = n0 < p.dv;                  // dim_v is a multiple of 16
-    uint4* fs = (uint4*) (sm + 2 * T::kStage + unit * kFrag);   // [DK / 16][2][32] S, then U e^(gc_63 - gc) [4][2][32]
-    uint4* fx = fs + DK / 16 * 2 * 32;                          // [4][2][32] X, then U
+    uint4* fs = (uint4*) (sm + 2 * T::kStage + unit * kFrag);   // S [DK / 16][2][32]; later U e^(gc_63 - gc) [4][2][32]
+    uint4* fu = fs + 256;                                       // U [4][2][32]
+    uint4* fx = fs + 512;                                       // X [4][2][32]
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], UN * W);
         fence_mbar_init();
@@ -614,23 +689,16 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaPa
         for (int e = 0; e < 4; ++e)
             S[i][e] = st >= 0 && in ? p.s_in[base + (int64_t) (i * 8 + 2 * qd + (e & 1)) * p.dv + g + (e >> 1) * 8] : 0.0f;
 
-    // The largest magnitudes of the unit's rows g and g + 8 from this warp's; `slot` alternates between exchanges.
-    auto row_peak = [&](float& a, float& c, int kind) {
-        a = quad_max(a), c = quad_max(c);
-        if (W == 2) {
-            if (qd == 0) peaks[unit][kind][part][0][g] = a, peaks[unit][kind][part][0][g + 8] = c;
-        }
+    auto split_a = [&](const float (&x)[4], const float (&y)[4], const RowScale& r, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+        split_f16x2(x[0], x[1], r.u[0], hi[0], lo[0]);
+        split_f16x2(x[2], x[3], r.u[1], hi[1], lo[1]);
+        split_f16x2(y[0], y[1], r.u[0], hi[2], lo[2]);
+        split_f16x2(y[2], y[3], r.u[1], hi[3], lo[3]);
     };
-    auto join_peak = [&](float& a, float& c, int kind) {
-        if (W == 2) a = fmaxf(a, peaks[unit][kind][part ^ (W - 1)][0][g]), c = fmaxf(c, peaks[unit][kind][part ^ (W - 1)][0][g + 8]);
-    };
-    auto split_a = [&](const float (&x)[4], const float (&y)[4], float u0, float u1, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
-        split_f16(x[0] * u0, x[1] * u0, hi[0], lo[0]);
-        split_f16(x[2] * u1, x[3] * u1, hi[1], lo[1]);
-        split_f16(y[0] * u0, y[1] * u0, hi[2], lo[2]);
-        split_f16(y[2] * u1, y[3] * u1, hi[3], lo[3]);
-    };
-    auto put = [&](uint4* f, int d, const uint32_t (&hi)[4], const uint32_t (&lo)[4]) {
+    // a row's part of a left operand (depth d of 16) into the unit's exchange, and out of it
+    auto put = [&](uint4* f, int d, const float (&x)[4], const float (&y)[4], const RowScale& r) {
+        uint32_t hi[4], lo[4];
+        split_a(x, y, r, hi, lo);
         f[(d * 2) * 32 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         f[(d * 2 + 1) * 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     };
@@ -639,60 +707,89 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaPa
         hi[0] = a.x, hi[1] = a.y, hi[2] = a.z, hi[3] = a.w;
         lo[0] = c.x, lo[1] = c.y, lo[2] = c.z, lo[3] = c.w;
     };
-    float su[2], si[2];                          // S's row scales and their inverses
-    auto scale_state = [&]() {
-        float a = 0.0f, c = 0.0f;
+    // largest magnitudes of the rows g and g + 8 in the warp's part, for the unit's other warps
+    auto tell_peak = [&](float& a, float& c, int kind) {
+        a = quad_max(a), c = quad_max(c);
+        if (W > 1 && qd == 0) peaks[unit][kind][part][g] = a, peaks[unit][kind][part][g + 8] = c;
+    };
+    auto join_peak = [&](float& a, float& c, int kind) {
+        if constexpr (W > 1) {
+#pragma unroll
+            for (int w = 0; w < W; ++w) a = fmaxf(a, peaks[unit][kind][w][g]), c = fmaxf(c, peaks[unit][kind][w][g + 8]);
+        }
+    };
+    RowScale rs, rx, ru, rf;                     // of S, X, U and U e^(gc_63 - gc)
+    auto state_peak = [&](float& a, float& c) {
+        a = c = 0.0f;
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
             a = fmaxf(a, fmaxf(fabsf(S[i][0]), fabsf(S[i][1])));
             c = fmaxf(c, fmaxf(fabsf(S[i][2]), fabsf(S[i][3])));
         }
-        row_peak(a, c, 0);
-        if (W == 2) pair_sync(1 + unit);
-        join_peak(a, c, 0);
-        pow2_scale(a, su[0], si[0]);
-        pow2_scale(c, su[1], si[1]);
-        if (W == 2) {
+    };
+    auto put_state = [&]() {
 #pragma unroll
-            for (int d = 0; d < NK / 2; ++d) {
-                uint32_t hi[4], lo[4];
-                split_a(S[2 * d], S[2 * d + 1], su[0], su[1], hi, lo);
-                put(fs, part * (NK / 2) + d, hi, lo);
+        for (int d = 0; d < NK / 2; ++d) put(fs, part * (NK / 2) + d, S[2 * d], S[2 * d + 1], rs);
+    };
+    auto share_state = [&]() {
+        float a, c;
+        state_peak(a, c);
+        tell_peak(a, c, 0);
+        if constexpr (W == 1) {
+            rs.set(a, c);
+        } else {
+            put_state();
+            unit_sync<W>(unit);
+            join_peak(a, c, 0);
+            if (!__all_sync(0xffffffffu, rs.holds(a, c))) {      // the same in every warp of the unit
+                rs.set(a, c);
+                unit_sync<W>(unit);
+                put_state();
+                unit_sync<W>(unit);
             }
-            pair_sync(1 + unit);
         }
     };
-    float V[NP * 2][4];
+    // the values of the unit's columns, as the inputs hold them until they are used
+    using Raw = std::conditional_t<E == E_F32, float, uint16_t>;
+    Raw V[NP * 2][4];
+    const Raw* vp = (const Raw*) p.v + (int64_t) h * p.v_head + n0 + g;
+    using Out = Elem<E>;
+    Out* op = (Out*) p.o + (int64_t) h * p.o_head + n0 + g;
     auto load_values = [&](int c) {
-        const int live = min(kChunk, s.n - c * kChunk);
-        const int64_t tok0 = s.tok + (int64_t) c * kChunk;
+        const int live = in ? min(kChunk, s.n - c * kChunk) : 0;
+        const Raw* r0 = vp + (s.tok + (int64_t) c * kChunk + 2 * qd) * p.v_tok;
 #pragma unroll
-        for (int x = 0; x < NP * 2; ++x)
+        for (int x = 0; x < NP; ++x) {
+            const Raw* r = r0 + tile_of(x) * 16 * p.v_tok;
+            const Raw* rows[2][2] = {{r, r + p.v_tok}, {r + 8 * p.v_tok, r + 9 * p.v_tok}};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int t = tile_of(x >> 1) * 16 + (x & 1) * 8 + 2 * qd + (e & 1);
-                V[x][e] = in && t < live ? load_t<E>(p.v, (tok0 + t) * p.v_tok + (int64_t) h * p.v_head + n0 + g + (e >> 1) * 8) : 0.0f;
-            }
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    V[2 * x + y][e] = tile_of(x) * 16 + 2 * qd + 8 * y + (e & 1) < live ? rows[y][e & 1][(e >> 1) * 8] : Raw(0);
+        }
+    };
+    auto value = [&](Raw r) -> float {
+        if constexpr (E == E_F32) return r;
+        else if constexpr (E == E_F16) return __half2float(__ushort_as_half(r));
+        else return __uint_as_float((uint32_t) r << 16);
     };
     if (chunks > 0) load_values(0);
-    scale_state();
+    share_state();
 
-    const int br = (lane & 7) + (lane >> 4) * 8, bp = (lane >> 3) & 1;      // right operand by rows
-    const int tr = (lane & 7) + ((lane >> 3) & 1) * 8, tp = lane >> 4;      // and transposed
+    // byte offsets of a lane's ldmatrix rows: right operands by rows (16 tokens a load) and transposed (keys); the
+    // piece of depth d or key tile n is an xor with 32 d or 32 n
+    const int br = (lane & 7) + (lane >> 4) * 8, tr = (lane & 7) + ((lane >> 3) & 1) * 8;
+    const uint32_t row_x = (((lane >> 3) & 1) ^ (br & 7)) << 4, col_x = ((lane >> 4) ^ (tr & 7)) << 4;
     bool ok = true;
     for (int c = 0; c < chunks; ++c) {
         const int i = c & 1;
         const int64_t tok0 = s.tok + (int64_t) c * kChunk;
-        const int live = min(kChunk, s.n - c * kChunk);
-        if (!mbar_wait_bounded(&full[i], (c >> 1) & 1, p.err, kSiteDelta)) ok = false;
-        if (W == 1) ok = __all_sync(0xffffffffu, ok);
-        else {                                    // the unit's warps leave together
-            if (lane == 0) peaks[unit][1][part][1][0] = ok ? 1.0f : 0.0f;
-            pair_sync(1 + unit);
-            ok = peaks[unit][1][0][1][0] != 0.0f && peaks[unit][1][W - 1][1][0] != 0.0f;
-        }
-        if (!ok) break;
-        const uint32_t kt = smem_u32(sm + i * T::kStage), qt = kt + PL * T::kTile, mt = kt + T::kHead, pt = mt + 2 * T::kSq;
+        const int live = in ? min(kChunk, s.n - c * kChunk) : 0;
+        // after a wait that gave up the loop runs on over whatever the tiles hold, so that every barrier is met
+        if (ok) ok = mbar_wait_bounded(&full[i], (c >> 1) & 1, p.err, kSiteDelta);
+        const uint32_t kt = smem_u32(sm + i * T::kStage), mt = kt + T::kHead;
+        const uint32_t kr = kt + br * RB, mr = mt + br * SB, kc = kt + tr * RB;
         const float* vec = (const float*) (sm + i * T::kStage + T::kHead + (2 + T::PP) * T::kSq);
 
         float Y[NP * 2][4], Z[NP * 2][4];
@@ -703,15 +800,15 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaPa
 #pragma unroll
         for (int d = 0; d < DK / 16; ++d) {
             uint32_t hi[4], lo[4], rk[NP][PL][4], rq[NP][PL][4];
+            const uint32_t at = kr + (row_x ^ (32 * d));
 #pragma unroll
             for (int n = 0; n < NP; ++n)
 #pragma unroll
                 for (int l = 0; l < PL; ++l) {
-                    const uint32_t at = l * T::kTile + swz(tile_of(n) * 16 + br, 2 * d + bp, DK * 2);
-                    ldsm4(rk[n][l], kt + at);
-                    ldsm4(rq[n][l], qt + at);
+                    ldsm4(rk[n][l], at + tile_of(n) * 16 * RB + l * T::kTile);
+                    ldsm4(rq[n][l], at + tile_of(n) * 16 * RB + (PL + l) * T::kTile);
                 }
-            if constexpr (W == 1) split_a(S[2 * d], S[2 * d + 1], su[0], su[1], hi, lo);
+            if constexpr (W == 1) split_a(S[2 * d], S[2 * d + 1], rs, hi, lo);
             else get(fs, d, hi, lo);
 #pragma unroll
             for (int l = 0; l < PL; ++l)
@@ -737,32 +834,32 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaPa
         for (int n = 0; n < NP * 2; ++n) {
             const int t = tile_of(n >> 1) * 16 + (n & 1) * 8 + 2 * qd;
             const float2 ek = *(const float2*) (vec + V_EK + t), eq = *(const float2*) (vec + V_EQ + t);
-            Y[n][0] = fmaf(-ek.x * si[0], Y[n][0], V[n][0]), Y[n][1] = fmaf(-ek.y * si[0], Y[n][1], V[n][1]);
-            Y[n][2] = fmaf(-ek.x * si[1], Y[n][2], V[n][2]), Y[n][3] = fmaf(-ek.y * si[1], Y[n][3], V[n][3]);
-            Z[n][0] *= eq.x * si[0], Z[n][1] *= eq.y * si[0], Z[n][2] *= eq.x * si[1], Z[n][3] *= eq.y * si[1];
+            Y[n][0] = fmaf(-ek.x * rs.i[0], Y[n][0], value(V[n][0])), Y[n][1] = fmaf(-ek.y * rs.i[0], Y[n][1], value(V[n][1]));
+            Y[n][2] = fmaf(-ek.x * rs.i[1], Y[n][2], value(V[n][2])), Y[n][3] = fmaf(-ek.y * rs.i[1], Y[n][3], value(V[n][3]));
+            Z[n][0] *= eq.x * rs.i[0], Z[n][1] *= eq.y * rs.i[0], Z[n][2] *= eq.x * rs.i[1], Z[n][3] *= eq.y * rs.i[1];
             a = fmaxf(a, fmaxf(fabsf(Y[n][0]), fabsf(Y[n][1])));
             cc = fmaxf(cc, fmaxf(fabsf(Y[n][2]), fabsf(Y[n][3])));
         }
         if (c + 1 < chunks) load_values(c + 1);   // they arrive during the rest of this chunk
 
-        float xu[2], xi[2];
-        row_peak(a, cc, 1);
-        if (W == 2) pair_sync(1 + unit);
-        join_peak(a, cc, 1);
-        pow2_scale(a, xu[0], xi[0]);
-        pow2_scale(cc, xu[1], xi[1]);
-        uint32_t xh[4][4], xl[4][4];               // X's left operands, all token tiles
+        uint32_t xh[4][4], xl[4][4];               // X's left operands, all token tiles; then U's
+        tell_peak(a, cc, 1);
         if constexpr (W == 1) {
+            rx.set(a, cc);
 #pragma unroll
-            for (int d = 0; d < 4; ++d) split_a(Y[2 * d], Y[2 * d + 1], xu[0], xu[1], xh[d], xl[d]);
+            for (int d = 0; d < 4; ++d) split_a(Y[2 * d], Y[2 * d + 1], rx, xh[d], xl[d]);
         } else {
 #pragma unroll
-            for (int n = 0; n < NP; ++n) {
-                uint32_t hi[4], lo[4];
-                split_a(Y[2 * n], Y[2 * n + 1], xu[0], xu[1], hi, lo);
-                put(fx, tile_of(n), hi, lo);
+            for (int n = 0; n < NP; ++n) put(fx, tile_of(n), Y[2 * n], Y[2 * n + 1], rx);
+            unit_sync<W>(unit);
+            join_peak(a, cc, 1);
+            if (!__all_sync(0xffffffffu, rx.holds(a, cc))) {
+                rx.set(a, cc);
+                unit_sync<W>(unit);
+#pragma unroll
+                for (int n = 0; n < NP; ++n) put(fx, tile_of(n), Y[2 * n], Y[2 * n + 1], rx);
+                unit_sync<W>(unit);
             }
-            pair_sync(1 + unit);
 #pragma unroll
             for (int d = 0; d < 4; ++d) get(fx, d, xh[d], xl[d]);
         }
@@ -772,94 +869,102 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaPa
 #pragma unroll
             for (int e = 0; e < 4; ++e) U[n][e] = 0.0f;
 #pragma unroll
-        for (int d = 0; d < 4; ++d)
+        for (int d = 0; d < 4; ++d) {
+            uint32_t r[NP][4], w[NP][4];
+            const uint32_t at = mr + (row_x ^ (32 * d));
 #pragma unroll
             for (int n = 0; n < NP; ++n) {
                 if (d > tile_of(n)) continue;      // M is lower triangular
-                uint32_t r[4], w[4];
-                const uint32_t at = swz(tile_of(n) * 16 + br, 2 * d + bp, kChunk * 2);
-                ldsm4(r, mt + at);
-                ldsm4(w, mt + T::kSq + at);
-                mma_f16(U[2 * n], xh[d], r[0], r[1]);
-                mma_f16(U[2 * n + 1], xh[d], r[2], r[3]);
-                mma_f16(U[2 * n], xl[d], r[0], r[1]);
-                mma_f16(U[2 * n + 1], xl[d], r[2], r[3]);
-                mma_f16(U[2 * n], xh[d], w[0], w[1]);
-                mma_f16(U[2 * n + 1], xh[d], w[2], w[3]);
+                ldsm4(r[n], at + tile_of(n) * 16 * SB);
+                ldsm4(w[n], at + tile_of(n) * 16 * SB + T::kSq);
             }
+#pragma unroll
+            for (int x = 0; x < 3; ++x)
+#pragma unroll
+                for (int n = 0; n < NP; ++n) {
+                    if (d > tile_of(n)) continue;
+                    mma_f16(U[2 * n], x == 1 ? xl[d] : xh[d], x == 2 ? w[n][0] : r[n][0], x == 2 ? w[n][1] : r[n][1]);
+                    mma_f16(U[2 * n + 1], x == 1 ? xl[d] : xh[d], x == 2 ? w[n][2] : r[n][2], x == 2 ? w[n][3] : r[n][3]);
+                }
+        }
         float F[NP * 2][4];                         // U e^(gc_63 - gc) by K's row scale
         float ua = 0.0f, uc = 0.0f, fa = 0.0f, fc = 0.0f;
 #pragma unroll
         for (int n = 0; n < NP * 2; ++n) {
             const int t = tile_of(n >> 1) * 16 + (n & 1) * 8 + 2 * qd;
             const float2 fm = *(const float2*) (vec + V_FM + t), ed = *(const float2*) (vec + V_ED + t);
-            U[n][0] *= fm.x * xi[0], U[n][1] *= fm.y * xi[0], U[n][2] *= fm.x * xi[1], U[n][3] *= fm.y * xi[1];
+            U[n][0] *= fm.x * rx.i[0], U[n][1] *= fm.y * rx.i[0], U[n][2] *= fm.x * rx.i[1], U[n][3] *= fm.y * rx.i[1];
             F[n][0] = U[n][0] * ed.x, F[n][1] = U[n][1] * ed.y, F[n][2] = U[n][2] * ed.x, F[n][3] = U[n][3] * ed.y;
             ua = fmaxf(ua, fmaxf(fabsf(U[n][0]), fabsf(U[n][1]))), uc = fmaxf(uc, fmaxf(fabsf(U[n][2]), fabsf(U[n][3])));
             fa = fmaxf(fa, fmaxf(fabsf(F[n][0]), fabsf(F[n][1]))), fc = fmaxf(fc, fmaxf(fabsf(F[n][2]), fabsf(F[n][3])));
         }
-        float uu[2], ui[2], fu[2], fi[2];
-        row_peak(ua, uc, 0);
-        fa = quad_max(fa), fc = quad_max(fc);
-        if (W == 2) {
-            if (qd == 0) peaks[unit][0][part][1][g] = fa, peaks[unit][0][part][1][g + 8] = fc;
-            pair_sync(1 + unit);
-            fa = fmaxf(fa, peaks[unit][0][part ^ (W - 1)][1][g]), fc = fmaxf(fc, peaks[unit][0][part ^ (W - 1)][1][g + 8]);
-        }
-        join_peak(ua, uc, 0);
-        pow2_scale(ua, uu[0], ui[0]);
-        pow2_scale(uc, uu[1], ui[1]);
-        pow2_scale(fa, fu[0], fi[0]);
-        pow2_scale(fc, fu[1], fi[1]);
         uint32_t fh[4][4], fl[4][4];
+        tell_peak(ua, uc, 2);
+        tell_peak(fa, fc, 3);
         if constexpr (W == 1) {
+            ru.set(ua, uc);
+            rf.set(fa, fc);
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
-                split_a(U[2 * d], U[2 * d + 1], uu[0], uu[1], xh[d], xl[d]);
-                split_a(F[2 * d], F[2 * d + 1], fu[0], fu[1], fh[d], fl[d]);
+                split_a(U[2 * d], U[2 * d + 1], ru, xh[d], xl[d]);
+                split_a(F[2 * d], F[2 * d + 1], rf, fh[d], fl[d]);
             }
         } else {
+            auto put_u = [&]() {
 #pragma unroll
-            for (int n = 0; n < NP; ++n) {
-                uint32_t hi[4], lo[4];
-                split_a(U[2 * n], U[2 * n + 1], uu[0], uu[1], hi, lo);
-                put(fx, tile_of(n), hi, lo);
-                split_a(F[2 * n], F[2 * n + 1], fu[0], fu[1], hi, lo);
-                put(fs, tile_of(n), hi, lo);
+                for (int n = 0; n < NP; ++n) {
+                    put(fu, tile_of(n), U[2 * n], U[2 * n + 1], ru);
+                    put(fs, tile_of(n), F[2 * n], F[2 * n + 1], rf);
+                }
+            };
+            put_u();
+            unit_sync<W>(unit);
+            join_peak(ua, uc, 2);
+            join_peak(fa, fc, 3);
+            if (!__all_sync(0xffffffffu, ru.holds(ua, uc) && rf.holds(fa, fc))) {
+                ru.set(ua, uc);
+                rf.set(fa, fc);
+                unit_sync<W>(unit);
+                put_u();
+                unit_sync<W>(unit);
             }
-            pair_sync(1 + unit);
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
-                get(fx, d, xh[d], xl[d]);
                 get(fs, d, fh[d], fl[d]);
+                get(fu, d, xh[d], xl[d]);
             }
         }
-        // S^T, key tile by key tile: the scaled product is added in fp32
+        // S^T, two pairs of key tiles at a time (eight products in flight): the scaled product is added in fp32
         const float end = vec[V_END];
+        const float end_f[2] = {rf.i[0], rf.i[1]};
 #pragma unroll
-        for (int n = 0; n < NK / 2; ++n) {
-            float acc[2][4];
+        for (int n = 0; n < NK / 2; n += NS) {
+            float acc[2 * NS][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[0][e] = acc[1][e] = 0.0f;
+            for (int x = 0; x < 2 * NS; ++x)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[x][e] = 0.0f;
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
-                const uint32_t at = swz(d * 16 + tr, 2 * (part * (NK / 2) + n) + tp, DK * 2);
+                uint32_t r[NS][PL][4];
 #pragma unroll
-                for (int l = 0; l < PL; ++l) {
-                    uint32_t r[4];
-                    ldsm4_t(r, kt + l * T::kTile + at);
-                    mma_f16(acc[0], fh[d], r[0], r[1]);
-                    mma_f16(acc[1], fh[d], r[2], r[3]);
-                    if (l == 0) {
-                        mma_f16(acc[0], fl[d], r[0], r[1]);
-                        mma_f16(acc[1], fl[d], r[2], r[3]);
+                for (int y = 0; y < NS; ++y)
+#pragma unroll
+                    for (int l = 0; l < PL; ++l)
+                        ldsm4_t(r[y][l], kc + (col_x ^ (32 * (part * (NK / 2) + n + y))) + d * 16 * RB + l * T::kTile);
+#pragma unroll
+                for (int l = 0; l < PL + 1; ++l)
+#pragma unroll
+                    for (int y = 0; y < NS; ++y) {
+                        const int k = l == 2 ? 1 : 0;            // hi hi, lo hi, hi lo
+                        mma_f16(acc[2 * y], l == 1 ? fl[d] : fh[d], r[y][k * (PL - 1)][0], r[y][k * (PL - 1)][1]);
+                        mma_f16(acc[2 * y + 1], l == 1 ? fl[d] : fh[d], r[y][k * (PL - 1)][2], r[y][k * (PL - 1)][3]);
                     }
-                }
             }
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
+            for (int x = 0; x < 2 * NS; ++x)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) S[2 * n + x][e] = fmaf(acc[x][e], fi[e >> 1], S[2 * n + x][e] * end);
+                for (int e = 0; e < 4; ++e) S[2 * n + x][e] = fmaf(acc[x][e], end_f[e >> 1], S[2 * n + x][e] * end);
         }
         // O^T
         float O[NP * 2][4];
@@ -868,42 +973,50 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaPa
 #pragma unroll
             for (int e = 0; e < 4; ++e) O[n][e] = 0.0f;
 #pragma unroll
-        for (int d = 0; d < 4; ++d)
+        for (int d = 0; d < 4; ++d) {
+            const uint32_t at = mr + (row_x ^ (32 * d)) + 2 * T::kSq;
 #pragma unroll
             for (int n = 0; n < NP; ++n) {
                 if (d > tile_of(n)) continue;
                 uint32_t r[4];
-                const uint32_t at = swz(tile_of(n) * 16 + br, 2 * d + bp, kChunk * 2);
-                ldsm4(r, pt + at);
+                ldsm4(r, at + tile_of(n) * 16 * SB);
                 mma_f16(O[2 * n], xh[d], r[0], r[1]);
                 mma_f16(O[2 * n + 1], xh[d], r[2], r[3]);
                 if (OS) {
                     uint32_t w[4];
-                    ldsm4(w, pt + T::kSq + at);
+                    ldsm4(w, at + tile_of(n) * 16 * SB + T::kSq);
                     mma_f16(O[2 * n], xl[d], r[0], r[1]);
                     mma_f16(O[2 * n + 1], xl[d], r[2], r[3]);
                     mma_f16(O[2 * n], xh[d], w[0], w[1]);
                     mma_f16(O[2 * n + 1], xh[d], w[2], w[3]);
                 }
             }
+        }
+        {
+            Out* r0 = op + (tok0 + 2 * qd) * p.o_tok;
 #pragma unroll
-        for (int n = 0; n < NP * 2; ++n) {
-            const int t0 = tile_of(n >> 1) * 16 + (n & 1) * 8 + 2 * qd;
-            const float2 fp = *(const float2*) (vec + V_FP + t0);
+            for (int n = 0; n < NP * 2; ++n) {
+                const int t0 = tile_of(n >> 1) * 16 + (n & 1) * 8;
+                const float2 fp = *(const float2*) (vec + V_FP + t0 + 2 * qd);
+                Out* r = r0 + t0 * p.o_tok;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int t = t0 + (e & 1);
-                const float o = fmaf(O[n][e], (e & 1 ? fp.y : fp.x) * ui[e >> 1], Z[n][e]);
-                if (in && t < live) store_elem(p.o, (tok0 + t) * p.o_tok + (int64_t) h * p.o_head + n0 + g + (e >> 1) * 8, E, o);
+                for (int e = 0; e < 4; ++e) {
+                    const float o = fmaf(O[n][e], (e & 1 ? fp.y : fp.x) * ru.i[e >> 1], Z[n][e]);
+                    Out* at = (e & 1 ? r + p.o_tok : r) + (e >> 1) * 8;
+                    if (t0 + 2 * qd + (e & 1) < live) store_t<E>(at, o);
+                }
             }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[i]);
-        if (tid == 0 && c + 2 < chunks) {
-            if (mbar_wait_bounded(&empty[i], (c >> 1) & 1, p.err, kSiteDelta)) fetch(c + 2);
-            else ok = false;
+        if (tid == 0 && c + 2 < chunks && ok) {
+            ok = mbar_wait_bounded(&empty[i], (c >> 1) & 1, p.err, kSiteDelta);
+            if (ok) fetch(c + 2);
         }
-        if (c + 1 < chunks) scale_state();
+        if (c + 1 < chunks) {
+            unit_sync<W>(unit);                     // the exchange is read
+            share_state();
+        }
     }
     if (!ok) {                                  // let copies in flight land before the CTA's memory goes
         for (int i = 0; i < 2; ++i)
@@ -949,7 +1062,7 @@ int64_t chunk_bytes(const tsb_delta_desc* d) {
 template <int E, int DK, int W>
 int launch_scan(const DeltaParams& p, cudaStream_t st) {
     constexpr int un = W == 1 ? 8 : 2;
-    constexpr int sm = 2 * Tiles<E, DK>::kStage + (W == 1 ? 0 : un * (DK / 16 * 2 * 512 + 4 * 2 * 512));
+    constexpr int sm = 2 * Tiles<E, DK>::kStage + (W == 1 ? 0 : un * 12 * 1024);
     static_assert(sm <= 226 * 1024, "shared memory");
     if (cudaFuncSetAttribute(k_delta_scan<E, DK, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm) != cudaSuccess)
         return dcuda("gated_delta: shared memory");
@@ -959,7 +1072,7 @@ int launch_scan(const DeltaParams& p, cudaStream_t st) {
 template <int E, int DK>
 int launch_chunks(const DeltaParams& p, cudaStream_t st) {
     using T = Tiles<E, DK>;
-    constexpr int sm = (T::kVal > T::kHead ? T::kVal : T::kHead) + (2 * 64 * LA + 32 * 36) * 4;
+    constexpr int sm = (T::kVal > T::kHead ? T::kVal : T::kHead) + (64 * LA + 32 * 36) * 4;
     if (cudaFuncSetAttribute(k_delta_prepare<E, DK>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm) != cudaSuccess)
         return dcuda("gated_delta: shared memory");
     k_delta_prepare<E, DK><<<dim3((unsigned) p.max_chunks, p.hk), 128, sm, st>>>(p);
