@@ -347,11 +347,12 @@ struct AttnParams {
     int64_t table_stride;
     int width;
     const int32_t *lens, *cu;
-    int tiles;                       // 16-row tiles of the longest request
+    int tiles;                       // row tiles of the longest request
     // split over CTAs: steps before each request, partial rows
     int64_t* pre;                    // [n_req + 1]
-    float* part;                     // [2 * CTAs][16][D], then their maxima and sums [2 * CTAs][2][16]
+    float* part;                     // [2 * CTAs][8][D], then their maxima and sums [2 * CTAs][2][8]
     int n_cta;
+    bool wide_out;                   // 16-byte aligned output rows
 };
 
 struct Req {
@@ -370,12 +371,13 @@ __device__ __forceinline__ Req attn_req(const AttnParams& p, int r) {
     }
     return q;
 }
-// The steps [first, first + n) that the rows of tile rt see.
+// The steps [first, first + n) that the rows of tile rt (of TR rows) see.
+template <int TR>
 __device__ __forceinline__ void tile_steps(const AttnParams& p, const Req& q, int rt, int& first, int& n) {
-    const int rows = q.n * p.G, r0 = rt * 16;
+    const int rows = q.n * p.G, r0 = rt * TR;
     first = n = 0;
     if (r0 >= rows) return;
-    const int i0 = r0 / p.G, i1 = (min(r0 + 16, rows) - 1) / p.G;
+    const int i0 = r0 / p.G, i1 = (min(r0 + TR, rows) - 1) / p.G;
     const int hi = q.len - q.n + i1 + 1, lo = p.window > 0 ? max(0, q.len - q.n + i0 - p.window + 1) : 0;
     if (hi <= 0) return;
     first = lo / kStep;
@@ -387,313 +389,416 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-__device__ __forceinline__ uint4 ld_code16(const int8_t* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint2 ld_code8(const int8_t* p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
-}
-// Four codes (bytes biased by 128) as fp16 values, exactly: byte b under the high byte 0x64 is the fp16 number 1024 + b.
-__device__ __forceinline__ uint32_t half_pair(uint32_t biased, uint32_t sel) {
-    const uint32_t w = __byte_perm(biased, 0x64646464u, sel);
-    const __half2 r = __hsub2(*(const __half2*) &w, __floats2half2_rn(1152.0f, 1152.0f));
-    return *(const uint32_t*) &r;
+
+// Four value codes as fp16 operands, exactly: the byte with its top bit flipped (u = code + 128) under the high byte 0x64
+// is the number 1024 + u, and 1152 is subtracted.  Bytes 0, 2 and 1, 3 of a word as two pairs.
+__device__ __forceinline__ void code_pairs(uint32_t w, uint32_t& even, uint32_t& odd) {
+    constexpr uint32_t mask = 0x00ff00ffu, flip = 0x64806480u;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(even) : "r"(w), "r"(mask), "r"(flip));          // (w & mask) ^ flip
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(odd) : "r"(w >> 8), "r"(mask), "r"(flip));
+    const __half2 e = __hsub2(*(const __half2*) &even, *(const __half2*) &flip);
+    const __half2 o = __hsub2(*(const __half2*) &odd, *(const __half2*) &flip);
+    even = *(const uint32_t*) &e, odd = *(const uint32_t*) &o;
 }
 
-// The rows of one tile as left operands, in shared memory [SP][D / 16][32 lanes]: row values in fp16 after a power-of-two
-// scale that brings the row's largest magnitude to [1024, 2048) (rowf undoes it), as one fp16 value (SP 1: exact for
-// 16-bit inputs down to 2^-25 of the row's largest) or as two (SP 2, 22 bits, for fp32 inputs).  The order of the
-// contraction is the order in which a lane reads codes: 16 consecutive bytes are four depths of 16.
-template <int D, int SP>
-__device__ __forceinline__ void stage_rows(const AttnParams& p, const Req& q, int h, int rt, uint4* qf, float* rowf,
+// The rows of one tile as right operands for products with the int8 key codes as they are: a row is scaled by a power of
+// two to whole numbers of 23 bits, and these are split into signed bytes, most significant first: planes
+// [NB][3][D / 32][32 lanes] of 8 bytes.  Sums of int8 products are exact, so the score is that of the scaled query, within
+// 2^-23 of the row's largest value a term (two planes, 2^-15, showed in weights of far smaller keys).  rowf[i] undoes the
+// scale and holds the score's factor, whose sign the rows carry.  The order of the contraction is the order in which a lane
+// reads codes: its 16 consecutive bytes are two depths of 32.
+template <int D, int NB>
+__device__ __forceinline__ void stage_rows(const AttnParams& p, const Req& q, int h, int rt, uint8_t* qf, float* rowf,
                                            int warp, int n_warps, int lane) {
     const int rows = q.n * p.G;
-    for (int i = warp; i < 16; i += n_warps) {
-        const int row = rt * 16 + i;
-        float x[D / 32];
-        float peak = 0.0f;
+    constexpr int kPlane = D / 32 * 256, TR = 8 * NB;
+    for (int i0 = warp; i0 < TR; i0 += 2 * n_warps) {
+        float x[2][D / 32];
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-            x[j] = row < rows ? load_elem(p.q, (int64_t) (q.tok + row / p.G) * p.q_tok + (int64_t) (h * p.G + row % p.G) * p.q_head +
-                                                   j * 32 + lane,
-                                          p.type)
-                              : 0.0f;
-            peak = fmaxf(peak, fabsf(x[j]));
+        for (int k = 0; k < 2; ++k) {                    // two rows' loads at once
+            const int i = i0 + k * n_warps, row = rt * TR + i;
+            if (i < TR && row < rows) {
+                const int64_t at = (int64_t) (q.tok + row / p.G) * p.q_tok + (int64_t) (h * p.G + row % p.G) * p.q_head + lane;
+#pragma unroll
+                for (int j = 0; j < D / 32; ++j) x[k][j] = load_elem(p.q, at + j * 32, p.type);
+            } else {
+#pragma unroll
+                for (int j = 0; j < D / 32; ++j) x[k][j] = 0.0f;
+            }
         }
-        peak = warp_max(peak);
-        const int e = (int) ((__float_as_uint(peak) >> 23) & 255u);              // 2^(e - 127) <= peak
-        const int up = e == 0 || e == 255 ? 0 : min(max(137 - e, -126), 126);    // to [1024, 2048)
-        const float f = __uint_as_float((uint32_t) (127 + up) << 23);
-        if (lane == 0) rowf[i] = p.scale_log2 * __uint_as_float((uint32_t) (127 - up) << 23);
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-            // value d of row i: chunk d / 64, quad (d / 16) % 4, byte d % 16 -> depth byte / 4, register and half
-            const int d = j * 32 + lane, b = d & 15;
-            const int slot = ((d >> 6) * 4 + (b >> 2)) * 32 + (i & 7) * 4 + ((d >> 4) & 3);
-            const int at = ((b & 2) ? 4 : 0) + ((i & 8) ? 2 : 0) + (b & 1);      // half index in {a0, a1, a2, a3}
-            const float y = x[j] * f;
-            const __half hi = __float2half_rn(y);
-            ((__half*) (qf + slot))[at] = hi;
-            if (SP == 2) ((__half*) (qf + (D / 16) * 32 + slot))[at] = __float2half_rn(y - __half2float(hi));
+        for (int k = 0; k < 2; ++k) {
+            const int i = i0 + k * n_warps;
+            if (i >= TR) break;
+            float peak = 0.0f;
+            bool nan = false;
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) peak = fmaxf(peak, fabsf(x[k][j])), nan |= !(fabsf(x[k][j]) <= 3.4028235e38f);
+            peak = warp_max(peak);
+            nan = __any_sync(0xffffffffu, nan);
+            constexpr int top = 148;                     // to [2^21, 2^22): the planes' carries fit
+            const int e = min(max((int) (__float_as_uint(peak) >> 23) & 255, 22), 254);
+            const float up = copysignf(__uint_as_float((uint32_t) min(127 + top - e, 254) << 23), p.scale_log2);
+            const float back = __uint_as_float((uint32_t) max(e - (top - 127), 1) << 23);
+            uint8_t* base = qf + (i >> 3) * 3 * kPlane + (i & 7) * 32;
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+                // value d of row i: chunk d / 64, quad (d / 16) % 4, byte d % 16 -> depth byte / 8, its place there
+                const int d = j * 32 + lane, b = d & 15;
+                uint8_t* at = base + ((d >> 6) * 2 + (b >> 3)) * 256 + ((d >> 4) & 3) * 8 + (b & 7);
+                int v = __float2int_rn(x[k][j] * up);
+#pragma unroll
+                for (int l = 2; l >= 0; --l) {
+                    at[l * kPlane] = (uint8_t) v;
+                    v = (v - (int) (int8_t) v) >> 8;
+                }
+            }
+            if (lane == 0) rowf[i] = nan ? __uint_as_float(0x7fffffffu) : fabsf(p.scale_log2) * back;   // NaN or infinity: a NaN row
         }
     }
 }
 
-// A warp's running rows: row g = lane / 4 and row g + 8 of the tile, output columns as the lane's value bytes.
-template <int D>
+// A warp's running rows, NB groups of 8.  Lane (g, quad) holds rows 2 quad and 2 quad + 1 of a group and the output columns
+// whose codes it reads: tile j of 16 columns of the transposed product is the bytes 2 j, 2 j + 1 of every lane's piece.
+template <int D, int NB>
 struct Rows {
-    float o[D / 8][4];
-    float m[2], l[2];
+    float4 o[NB][D / 16];            // {column 2 j: row 2 quad, row + 1; column 2 j + 1: row 2 quad, row + 1}
+    float m[NB][2], l[NB][2];
     __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-        m[0] = m[1] = -INFINITY;
-        l[0] = l[1] = 0.0f;
-    }
-};
-
-template <int D>
-struct Codes {
-    static constexpr int KC = D / 64, VC = D / 128 > 0 ? D / 128 : 1;
-    uint4 k[2][KC], v[4][VC];
-    float ks, vs;
-};
-
-template <int D>
-__device__ __forceinline__ void load_k(Codes<D>& c, const Cache& cc, int64_t bh, int in, int lane) {
-    const int8_t* base = cc.k + (bh * cc.bs + in) * D + (lane >> 2) * D + (lane & 3) * 16;
+        for (int u = 0; u < NB; ++u) {
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-        for (int i = 0; i < Codes<D>::KC; ++i) c.k[nt][i] = ld_code16(base + nt * 8 * D + i * 64);
-    c.ks = __ldg(cc.ks + bh);
-}
-template <int D>
-__device__ __forceinline__ void load_v(Codes<D>& c, const Cache& cc, int64_t bh, int in, int lane) {
-    const int g = lane >> 2, q = lane & 3;
-    const int8_t* base = cc.v + (bh * cc.bs + in) * D;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const int8_t* row = base + (2 * q + (t & 1) + (t >> 1) * 8) * D;
-        if constexpr (D == 64) {
-            const uint2 w = ld_code8(row + g * 8);
-            c.v[t][0] = make_uint4(w.x, w.y, 0, 0);
-        } else {
-#pragma unroll
-            for (int i = 0; i < Codes<D>::VC; ++i) c.v[t][i] = ld_code16(row + i * 128 + g * 16);
+            for (int i = 0; i < D / 16; ++i) o[u][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            m[u][0] = m[u][1] = -INFINITY;
+            l[u][0] = l[u][1] = 0.0f;
         }
     }
-    c.vs = __ldg(cc.vs + bh);
+    // the first of 2 * (tiles) consecutive columns that tiles j, j + 1, .. hold
+    __device__ static __forceinline__ int column(int j, int g) { return D == 64 ? g * 8 + 2 * j : (j / 8) * 128 + g * 16 + 2 * (j % 8); }
+};
+
+constexpr float kShift = 15.0f;  // weights are exp2(x - the row's largest so far + 15): at most 2^15, and fp16 keeps 11 bits
+                                 // of those down to 2^-29 of the largest
+
+// A warp's ring of steps in shared memory: per step 16 tokens' key codes and their value codes, 16-byte pieces permuted so
+// that a quarter warp's reads touch every bank once, and {key scale, value scale, whether the block is in the cache}.
+// Depths by what fits the CTAs a SM holds: 80 to 130 KB a SM are in flight.
+//   head_dim 128, 256: piece ^ (2 ((row / 2) % 4) ^ 4 (row % 2)) within its 128 bytes
+//   head_dim 64: keys as they are; value rows in the order 0 2 4 6 1 3 5 7 (and + 8), piece ^ 2 (their place / 2 % 2)
+template <int D>
+struct Ring {
+    static constexpr int kDepth = D == 256 ? 2 : D == 128 ? 3 : 5;
+    static constexpr int kHalf = kStep * D;
+    static constexpr int kStage = 2 * kHalf;
+    static constexpr int kHeads = kDepth * kStage;
+    static constexpr int kBytes = kHeads + 128;
+    static constexpr int kRow1 = D == 64 ? 4 * D : D;      // from a lane's even value row to the odd one, before the xor
+    // byte offsets of 16-byte piece `lane` of a step (piece 32 i + lane: xor the rows' change, plus 512 i) ...
+    __device__ static __forceinline__ int put_k(int lane) {
+        const int row = lane / (D / 16), piece = lane % (D / 16);
+        return D == 64 ? lane * 16 : row * D + ((piece ^ swizzle(row)) << 4);
+    }
+    __device__ static __forceinline__ int put_v(int lane) {
+        if (D != 64) return put_k(lane);
+        const int row = lane >> 2, piece = lane & 3, at = ((row & 1) << 2) | (row >> 1);
+        return at * D + ((piece ^ (((at >> 1) & 1) << 1)) << 4);
+    }
+    // ... and of what lane (g, quad) reads: key row g, piece quad; value row 2 quad, piece g (D 64: half a piece)
+    __device__ static __forceinline__ int get_k(int g, int qd) {
+        return D == 64 ? g * D + qd * 16 : g * D + ((qd ^ swizzle(g)) << 4);
+    }
+    __device__ static __forceinline__ int get_v(int g, int qd) {
+        return D == 64 ? qd * D + (((g >> 1) ^ (((qd >> 1) & 1) << 1)) << 4) + (g & 1) * 8
+                       : 2 * qd * D + ((g ^ swizzle(2 * qd)) << 4);
+    }
+    __device__ static __forceinline__ int swizzle(int row) { return (((row >> 1) & 3) << 1) ^ ((row & 1) << 2); }
+};
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-constexpr float kShift = 15.0f;  // a step's weights are exp2(x - largest of the step + 15): at most 2^15, and fp16 keeps
-                                 // 11 bits of those down to 2^-29 of the step's largest
-constexpr float kLazy = 40.0f;   // a row's reference m moves when a step exceeds it by 2^40: fp32 holds the sums until then
+// A warp's walk over steps first + off, first + off + stride, ... below first + n of request r's keys and values, for one
+// tile of rows.  The constructor begins the copies (the rows need not be staged yet), run() does the rest.
+// Both products are transposed, keys and value columns as the 16 rows of the instruction and queries as its 8 columns: a
+// decode step has at most 8 rows a head in most models, and a tile of queries by 16 would be half empty, at twice the
+// products, registers and exponentials.  x = q . k (int8 products, exact) times the block's key scale and the row's; the
+// online softmax's largest score m and sum l in fp32 (the lanes compare their scores with m; only when one is larger do
+// they meet); o += weights . codes times the block's value scale.
+// SP 1, 16-bit outputs: weights, times 2^15 and the value scale relative to the largest so far, enter the product as one
+//   fp16 value (11 bits down to 2^-29 of the largest weight; 2^-40 of it below) and o accumulates in the tensor cores.
+// SP 2, fp32 outputs: weights as two fp16 values; a step's product starts from zero and is added in fp32 times the value
+//   scale, since the tensor cores' sums truncate.
+template <int D, int SP, int NB>
+struct Walk {
+    const AttnParams& p;
+    const int32_t* tab;
+    uint32_t ring, put_k, put_v;
+    int shift, first, n, stride, h, lane;
+    int s, s_copy, stage_copy, id_copy;
 
-// The tile's rows against steps first + off, first + off + stride, ... below first + n of request r's keys and values.
-// Per step of 16 tokens: x = q . k (fp16 products of exact codes, fp32 sums) times the block's key scale; weights
-// exp2(x - the row's largest x of the step); the row's sum l and outputs o in fp32 relative to exp2(m), m one of the
-// rows' earlier maxima: o = o + exp2(step's largest - m) * (block's value scale) * (weights . codes), where the product
-// of a step starts from zero, so the factors of a step are applied in fp32.  Weights enter the product as one fp16
-// value (SP 1: 2^-12 of each, averaged over the tokens, for 16-bit outputs) or as two (SP 2).
-// The next step's keys are loaded as soon as this step's are used, its values likewise, so that half of a step's
-// bytes are in flight at any time without a second set of registers.
-template <int D, int SP>
-__device__ __forceinline__ void attend(const AttnParams& p, const uint4* qf, const float* rowf, const Req& q, int r, int h,
-                                       int rt, int first, int n, int off, int stride, Rows<D>& R, int lane) {
-    const int g = lane >> 2, qd = lane & 3;
-    const int32_t* tab = p.table + (int64_t) r * p.table_stride;
-    const int per = p.c.bs / kStep;
-    int pos[2], low[2];              // a row sees the keys low .. pos
-    int pmin = INT_MAX, lmax = INT_MIN;
+    __device__ __forceinline__ Walk(const AttnParams& p, uint32_t ring, int r, int h, int first, int n, int off, int stride, int lane)
+        : p(p), tab(p.table + (int64_t) r * p.table_stride), ring(ring), put_k(Ring<D>::put_k(lane)),
+          put_v(Ring<D>::kHalf + Ring<D>::put_v(lane)), shift(p.c.bs >> 6 ? 2 : p.c.bs >> 5), first(first), n(n), stride(stride), h(h),
+          lane(lane), s(off), s_copy(off), stage_copy(0) {
+        id_copy = block(s_copy);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int row = rt * 16 + g + 8 * i, rows = q.n * p.G;
-        pos[i] = q.len - q.n + min(row, rows - 1) / p.G;
-        low[i] = p.window > 0 ? pos[i] - p.window + 1 : INT_MIN;
+        for (int i = 0; i < Ring<D>::kDepth - 1; ++i) copy();
     }
-    {
-        const int rows = q.n * p.G;
-        pmin = q.len - q.n + (rt * 16) / p.G;
-        const int pmax = q.len - q.n + (min(rt * 16 + 16, rows) - 1) / p.G;
-        lmax = p.window > 0 ? pmax - p.window + 1 : INT_MIN;
+    __device__ __forceinline__ int block(int x) const { return x < n ? __ldg(tab + ((first + x) >> shift)) : 0; }
+    // the next step's codes and scales on their way (one group, empty past the last step)
+    __device__ __forceinline__ void copy() {
+        if (s_copy < n) {
+            const bool ok = id_copy >= 0 && id_copy < p.c.n_blocks;
+            const int64_t bh = (int64_t) (ok ? id_copy : 0) * p.c.H + h;
+            const int64_t at = (bh * p.c.bs + (((first + s_copy) & ((1 << shift) - 1)) * kStep)) * D + lane * 16;
+            const uint32_t dst = ring + stage_copy * Ring<D>::kStage, head = ring + Ring<D>::kHeads + stage_copy * 16;
+            const uint32_t k0 = dst + put_k, v0 = dst + put_v;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                const uint32_t x = D == 256 ? 32 * (i & 3) : D == 128 ? 64 * (i & 1) : 0;
+                cp_async16((k0 ^ x) + i * 512, p.c.k + at + i * 512);
+                cp_async16((v0 ^ x) + i * 512, p.c.v + at + i * 512);
+            }
+            if (lane == 0) cp4(head, p.c.ks + bh);
+            if (lane == 1) cp4(head + 4, p.c.vs + bh);
+            if (lane == 2) asm volatile("st.shared.u32 [%0], %1;" ::"r"(head + 8), "r"((int) ok) : "memory");
+        }
+        cp_commit();
+        s_copy += stride;
+        id_copy = block(s_copy);
+        stage_copy = stage_copy + 1 == Ring<D>::kDepth ? 0 : stage_copy + 1;
     }
-    const float rf[2] = {rowf[g], rowf[g + 8]};
-    auto block = [&](int s) -> int {
-        const int b = s < n ? __ldg(tab + (first + s) / per) : -1;
-        return b < p.c.n_blocks ? b : -1;
-    };
-    Codes<D> c;
-    int s = off;
-    int id = block(s), id_next = block(s + stride);
-    if (id >= 0) {
-        const int64_t bh = (int64_t) id * p.c.H + h;
-        load_k<D>(c, p.c, bh, (first + s) % per * kStep, lane);
-        load_v<D>(c, p.c, bh, (first + s) % per * kStep, lane);
-    }
-    for (; s < n; s += stride) {
-        const int id_after = block(s + 2 * stride);
-        const int in_next = (first + s + stride) % per * kStep;
-        const int64_t bh_next = (int64_t) id_next * p.c.H + h;
-        float x[2][4];
-        if (id >= 0) {
+
+    __device__ __forceinline__ void run(const Req& q, int rt, const uint8_t* qf, const float* rowf, Rows<D, NB>& R) {
+        constexpr int TR = 8 * NB;
+        const int g = lane >> 2, qd = lane & 3, rows = q.n * p.G;
+        constexpr bool QREG = NB == 1 && D <= 128;       // the rows' operands stay in registers where they fit
+        const uint2* qp = (const uint2*) qf + lane;
+        uint2 qr[QREG ? 3 * D / 32 : 1];
+        if constexpr (QREG) {
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.0f;
+            for (int i = 0; i < 3 * D / 32; ++i) qr[i] = qp[i * 32];
+        }
+        const uint32_t get_k = Ring<D>::get_k(g, qd), get_v = Ring<D>::kHalf + Ring<D>::get_v(g, qd);
+        int pos[NB][2];                                  // a row sees the keys up to pos, the last `window` of them
+        float rf[NB][2];
 #pragma unroll
-            for (int i = 0; i < Codes<D>::KC; ++i) {
+        for (int u = 0; u < NB; ++u)
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
-                    const uint4 a4 = qf[(i * 4 + kk) * 32 + lane];
-                    const uint32_t a[4] = {a4.x, a4.y, a4.z, a4.w};
-                    uint32_t b[4] = {0, 0, 0, 0};
-                    if (SP == 2) {
-                        const uint4 b4 = qf[(D / 16 + i * 4 + kk) * 32 + lane];
-                        b[0] = b4.x, b[1] = b4.y, b[2] = b4.z, b[3] = b4.w;
-                    }
+            for (int i = 0; i < 2; ++i) {
+                pos[u][i] = q.len - q.n + min(rt * TR + u * 8 + 2 * qd + i, rows - 1) / p.G;
+                rf[u][i] = rowf[u * 8 + 2 * qd + i];
+            }
+        const int pmin = q.len - q.n + (rt * TR) / p.G;
+        const int lmax = p.window > 0 ? q.len - q.n + (min(rt * TR + TR, rows) - 1) / p.G - p.window + 1 : INT_MIN;
+        float ref = 0.0f, per_ref = 0.0f;                // SP 1: a power of two above the value scales so far, its inverse
+        int stage = 0;
+        for (; s < n; s += stride) {
+            __syncwarp();                                // the stage that copy() fills is read
+            copy();
+            cp_wait<Ring<D>::kDepth - 1>();
+            __syncwarp();
+            const uint32_t at = ring + stage * Ring<D>::kStage;
+            const uint4 head = lds16(ring + Ring<D>::kHeads + stage * 16);
+            stage = stage + 1 == Ring<D>::kDepth ? 0 : stage + 1;
+            if (head.z == 0) continue;                   // a block outside the cache
+            const float ks = __uint_as_float(head.x), vs = __uint_as_float(head.y);
+
+            int xi[NB][3][4];
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) {
-                        const uint32_t w = (kk == 0 ? c.k[nt][i].x : kk == 1 ? c.k[nt][i].y : kk == 2 ? c.k[nt][i].z : c.k[nt][i].w) ^ 0x80808080u;
-                        const uint32_t b0 = half_pair(w, 0x4140), b1 = half_pair(w, 0x4342);
-                        mma_f16(x[nt], a, b0, b1);
-                        if (SP == 2) mma_f16(x[nt], b, b0, b1);
-                    }
+            for (int i = 0; i < D / 64; ++i) {
+                const uint32_t ka = ((at + get_k) ^ ((i & 1) * 64)) + (i >> 1) * 128;
+                const uint4 k0 = lds16(ka), k1 = lds16(ka + 8 * D);
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk) {
+                    const uint32_t a[4] = {word(k0, 2 * kk), word(k1, 2 * kk), word(k0, 2 * kk + 1), word(k1, 2 * kk + 1)};
+#pragma unroll
+                    for (int u = 0; u < NB; ++u)
+#pragma unroll
+                        for (int l = 0; l < 3; ++l) {
+                            const uint2 b = QREG ? qr[QREG ? l * (D / 32) + i * 2 + kk : 0] : qp[(u * 3 * (D / 32) + l * (D / 32) + i * 2 + kk) * 32];
+                            if (i == 0 && kk == 0) mma_s8_zero(xi[u][l], a, b.x, b.y);
+                            else mma_s8(xi[u][l], a, b.x, b.y);
+                        }
                 }
             }
-        }
-        const float ks = c.ks;
-        if (id_next >= 0) load_k<D>(c, p.c, bh_next, in_next, lane);
-        if (id >= 0) {
+            // y[e]: token g + 8 (e / 2), row 2 quad + e % 2
+            float y[NB][4], sc[NB][2];
             const int t0 = (first + s) * kStep;
             const bool edge = t0 + kStep - 1 > pmin || t0 < lmax;
+            bool moved = SP == 1 && vs > ref;
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
+            for (int u = 0; u < NB; ++u) {
+                sc[u][0] = ks * rf[u][0], sc[u][1] = ks * rf[u][1];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int i = e >> 1, t = t0 + nt * 8 + 2 * qd + (e & 1);
-                    x[nt][e] *= ks * rf[i];
-                    if (edge && (t > pos[i] || t < low[i])) x[nt][e] = -INFINITY;
-                }
-            float mx[2], al[2], f[2];
-            bool moved = false;
+                for (int e = 0; e < 4; ++e) y[u][e] = fmaf((float) xi[u][0][e], 65536.0f, (float) (xi[u][1][e] * 256 + xi[u][2][e])) * sc[u][e & 1];
+                if (edge) {
+                    const int w = p.window > 0 ? p.window : INT_MAX;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                mx[i] = fmaxf(fmaxf(x[0][2 * i], x[0][2 * i + 1]), fmaxf(x[1][2 * i], x[1][2 * i + 1]));
-                mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-                mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-                al[i] = 1.0f;
-                if (mx[i] > R.m[i] + kLazy) {        // true for the first key of a row (m = -inf)
-                    al[i] = ex2(R.m[i] - mx[i]);
-                    R.m[i] = mx[i];
-                    moved = true;
-                }
-                f[i] = mx[i] == -INFINITY ? 0.0f : ex2(mx[i] - R.m[i]);
-            }
-            if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-                for (int j = 0; j < D / 8; ++j) {
-                    R.o[j][0] *= al[0], R.o[j][1] *= al[0];
-                    R.o[j][2] *= al[1], R.o[j][3] *= al[1];
-                }
-                R.l[0] *= al[0], R.l[1] *= al[1];
-            }
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float z = mx[i] == -INFINITY ? 0.0f : mx[i] - kShift;
-                float sum = 0.0f;
-#pragma unroll
-                for (int nt = 0; nt < 2; ++nt) {
-                    const float p0 = ex2(x[nt][2 * i] - z), p1 = ex2(x[nt][2 * i + 1] - z);
-                    sum += p0 + p1;
-                    const uint32_t u = pack_f16(p0, p1);
-                    hi[nt * 2 + i] = u;
-                    if (SP == 2) {
-                        const float2 w = __half22float2(*(const __half2*) &u);
-                        lo[nt * 2 + i] = pack_f16(p0 - w.x, p1 - w.y);
+                    for (int e = 0; e < 4; ++e) {
+                        const int t = t0 + g + 8 * (e >> 1);
+                        if (t > pos[u][e & 1] || pos[u][e & 1] - t >= w) y[u][e] = -INFINITY;
                     }
                 }
-                R.l[i] = fmaf(sum, f[i], R.l[i]);
+                moved |= fmaxf(y[u][0], y[u][2]) > R.m[u][0] || fmaxf(y[u][1], y[u][3]) > R.m[u][1];
             }
-            f[0] *= c.vs, f[1] *= c.vs;
+            if (__any_sync(0xffffffffu, moved)) {
+                float by = 1.0f;
+                if (SP == 1 && vs > ref) {
+                    const uint32_t e = max(min((__float_as_uint(vs) >> 23) + 1, 253u), 2u);      // 2^(e - 127) > vs
+                    by = ref * __uint_as_float((254 - e) << 23);
+                    ref = __uint_as_float(e << 23), per_ref = __uint_as_float((254 - e) << 23);
+                }
 #pragma unroll
-            for (int i = 0; i < Codes<D>::VC; ++i) {
+                for (int u = 0; u < NB; ++u) {
+                    float al[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float mx = fmaxf(R.m[u][i], fmaxf(y[u][i], y[u][2 + i]));
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                        al[i] = mx == -INFINITY ? 1.0f : ex2(R.m[u][i] - mx);
+                        R.m[u][i] = mx;
+                        R.l[u][i] *= al[i];
+                        al[i] *= by;
+                    }
+#pragma unroll
+                    for (int j = 0; j < D / 16; ++j) {
+                        R.o[u][j].x *= al[0], R.o[u][j].y *= al[1], R.o[u][j].z *= al[0], R.o[u][j].w *= al[1];
+                    }
+                }
+            }
+            uint32_t b[NB][2], bl[NB][2];
+            const float r = SP == 1 ? vs * per_ref : 1.0f;
+#pragma unroll
+            for (int u = 0; u < NB; ++u) {
+                const float z[2] = {R.m[u][0] == -INFINITY ? 0.0f : kShift - R.m[u][0], R.m[u][1] == -INFINITY ? 0.0f : kShift - R.m[u][1]};
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = ex2(y[u][e] + z[e & 1]);
+                R.l[u][0] += w[0] + w[2], R.l[u][1] += w[1] + w[3];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t hi = pack_f16(w[2 * e] * r, w[2 * e + 1] * r);
+                    b[u][e] = transpose8(hi);
+                    if (SP == 2) {
+                        const float2 f = __half22float2(*(const __half2*) &hi);
+                        bl[u][e] = transpose8(pack_f16(w[2 * e] - f.x, w[2 * e + 1] - f.y));
+                    }
+                }
+            }
+            const uint32_t va = at + get_v, vb = D == 64 ? va + Ring<D>::kRow1 : (va ^ 64) + Ring<D>::kRow1;
+#pragma unroll
+            for (int i = 0; i < (D + 127) / 128; ++i) {
+                uint4 v[4];                              // tokens 2 quad, 2 quad + 1, 2 quad + 8, 2 quad + 9
+                if constexpr (D == 64) {
+                    const uint2 a = lds8(va), c = lds8(vb), d = lds8(va + 8 * D), e = lds8(vb + 8 * D);
+                    v[0] = make_uint4(a.x, a.y, 0, 0), v[1] = make_uint4(c.x, c.y, 0, 0);
+                    v[2] = make_uint4(d.x, d.y, 0, 0), v[3] = make_uint4(e.x, e.y, 0, 0);
+                } else {
+                    v[0] = lds16(va + i * 128), v[1] = lds16(vb + i * 128);
+                    v[2] = lds16(va + i * 128 + 8 * D), v[3] = lds16(vb + i * 128 + 8 * D);
+                }
 #pragma unroll
                 for (int w = 0; w < (D == 64 ? 2 : 4); ++w) {
-                    uint32_t y[4];
+                    uint32_t c0[4], c1[4];               // bytes 0 .. 3 of the word: two tokens side by side, and eight on
+                    code_pairs(__byte_perm(word(v[0], w), word(v[1], w), 0x6420), c0[0], c0[2]);
+                    code_pairs(__byte_perm(word(v[0], w), word(v[1], w), 0x7531), c0[1], c0[3]);
+                    code_pairs(__byte_perm(word(v[2], w), word(v[3], w), 0x6420), c1[0], c1[2]);
+                    code_pairs(__byte_perm(word(v[2], w), word(v[3], w), 0x7531), c1[1], c1[3]);
 #pragma unroll
-                    for (int t = 0; t < 4; ++t)
-                        y[t] = (w == 0 ? c.v[t][i].x : w == 1 ? c.v[t][i].y : w == 2 ? c.v[t][i].z : c.v[t][i].w) ^ 0x80808080u;
-                    const uint32_t a01 = __byte_perm(y[0], y[1], 0x5140), a23 = __byte_perm(y[0], y[1], 0x7362);
-                    const uint32_t b01 = __byte_perm(y[2], y[3], 0x5140), b23 = __byte_perm(y[2], y[3], 0x7362);
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t a[4] = {c0[2 * j], c0[2 * j + 1], c1[2 * j], c1[2 * j + 1]};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t sel = j & 1 ? 0x4342 : 0x4140;
-                        const uint32_t b0 = half_pair(j < 2 ? a01 : a23, sel), b1 = half_pair(j < 2 ? b01 : b23, sel);
-                        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        mma_f16(acc, hi, b0, b1);
-                        if (SP == 2) mma_f16(acc, lo, b0, b1);
-                        float* o = R.o[(i * 4 + w) * 4 + j];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[e] = fmaf(f[e >> 1], acc[e], o[e]);
+                        for (int u = 0; u < NB; ++u) {
+                            float4& o = R.o[u][i * 8 + w * 2 + j];
+                            if constexpr (SP == 1) {
+                                mma_f16(o, a, b[u][0], b[u][1]);
+                            } else {
+                                float acc[4];
+                                mma_f16_zero(acc, a, b[u][0], b[u][1]);
+                                mma_f16(acc, a, bl[u][0], bl[u][1]);
+                                o.x = fmaf(vs, acc[0], o.x), o.y = fmaf(vs, acc[1], o.y);
+                                o.z = fmaf(vs, acc[2], o.z), o.w = fmaf(vs, acc[3], o.w);
+                            }
+                        }
                     }
                 }
             }
         }
-        if (id_next >= 0) load_v<D>(c, p.c, bh_next, in_next, lane);
-        id = id_next;
-        id_next = id_after;
-    }
-    // every lane of a row's four holds a part of its sum
+        cp_wait<0>();                                    // (only empty groups are left)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        R.l[i] += __shfl_xor_sync(0xffffffffu, R.l[i], 1);
-        R.l[i] += __shfl_xor_sync(0xffffffffu, R.l[i], 2);
+        for (int u = 0; u < NB; ++u) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {                // the lanes of a column hold parts of its row's sum
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) R.l[u][i] += __shfl_xor_sync(0xffffffffu, R.l[u][i], o);
+            }
+            if (SP == 1) {
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j) R.o[u][j].x *= ref, R.o[u][j].y *= ref, R.o[u][j].z *= ref, R.o[u][j].w *= ref;
+            }
+        }
+    }
+};
+
+// N values (2 at D 64, else a multiple of 4) to consecutive elements; `wide`: N elements are one aligned access.
+template <int N>
+__device__ __forceinline__ void store_row(void* o, int64_t at, int type, const float (&x)[N], bool wide) {
+    if (!wide) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) store_elem(o, at + i, type, x[i]);
+    } else if (type == E_F32) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) *(float2*) ((float*) o + at + i) = make_float2(x[i], x[i + 1]);
+    } else {
+        uint32_t u[N / 2];
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) u[i] = type == E_F16 ? pack_f16(x[2 * i], x[2 * i + 1]) : pack_bf16(x[2 * i], x[2 * i + 1]);
+        if constexpr (N >= 8) {
+#pragma unroll
+            for (int i = 0; i < N / 8; ++i) *((uint4*) ((uint16_t*) o + at) + i) = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+        } else if constexpr (N == 4) {
+            *(uint2*) ((uint16_t*) o + at) = make_uint2(u[0], u[1]);
+        } else {
+            *(uint32_t*) ((uint16_t*) o + at) = u[0];
+        }
     }
 }
 
-// Output tile j of a lane holds the columns col(j), col(j) + CW (its two accumulator columns); consecutive j are
-// consecutive columns, so a lane's 16 (D = 64: 8) values of a row half are consecutive.
 template <int D>
-__device__ __forceinline__ int out_col(int j, int half, int qd) {
-    constexpr int W = D == 64 ? 8 : 16;
-    return (j / W) * 128 + (2 * qd + half) * W + j % W;
-}
+constexpr int kSplitCtas = D == 256 ? 3 : D == 128 ? 4 : 5;   // CTAs a SM holds
 
-template <int D>
-__device__ __forceinline__ void write_rows(const AttnParams& p, const Req& q, int h, int rt, const Rows<D>& R, int lane) {
-    const int g = lane >> 2, qd = lane & 3, rows = q.n * p.G;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int row = rt * 16 + g + 8 * i;
-        if (row >= rows) continue;
-        const float inv = R.l[i] > 0.0f ? 1.0f / R.l[i] : 0.0f;      // a row that sees no key is zero
-        const int64_t base = (int64_t) (q.tok + row / p.G) * p.o_tok + (int64_t) (h * p.G + row % p.G) * p.o_head;
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int j = 0; j < D / 8; ++j)
-                store_elem(p.o, base + out_col<D>(j, half, qd), p.type, R.o[j][2 * i + half] * inv);
-    }
-}
-
-// The steps of all (request, head, tile) segments, one after the other (request, then head, then tile), are cut into
+// The steps of all (request, head, tile of 8 rows) segments, one after the other (request, then head, then tile), are cut into
 // equal ranges, one per CTA; a range's warps take its steps in turn and join their rows through shared memory at the
 // end of each segment.  A segment inside one range is finished there; one cut by a range's end leaves its rows, maxima
 // and sums for k_attn_join.  So a lone request of 131,072 tokens and 64 requests of uneven lengths fill the GPU alike.
 template <int D, int SP>
-__global__ void __launch_bounds__(kAttnWarps * 32) k_attn_split(const AttnParams p) {
-    extern __shared__ __align__(16) uint8_t smem[];
-    uint4* qf = (uint4*) smem;                                         // [SP][D / 16][32]
-    float* mrg = (float*) (smem + SP * (D / 16) * 32 * 16);            // [2][16][D] rows in transit between warps
-    float* ml = mrg + 2 * 16 * D;                                      // [2][2][16]
-    float* rowf = ml + 64;                                             // [16]
-    int64_t* pre = (int64_t*) (rowf + 16);                             // [n_req + 1]
+__global__ void __launch_bounds__(kAttnWarps * 32, kSplitCtas<D>) k_attn_split(const __grid_constant__ AttnParams p) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t* rings = smem;                                             // [warps] rings; then [warps][8][D] rows to join
+    float4* mrg = (float4*) rings;
+    uint8_t* qf = rings + kAttnWarps * Ring<D>::kBytes;                // [3][D / 32][32][8]
+    float* ml = (float*) (qf + 3 * (D / 32) * 256);                    // [warps][2][8]
+    float* rowf = ml + kAttnWarps * 16;                                // [8]
+    int64_t* pre = (int64_t*) (rowf + 8);                              // [n_req + 1]
+    static_assert(Ring<D>::kBytes >= 8 * D * 4, "the rows to join lie over the rings");
     __shared__ int64_t wsum[kAttnWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int R = p.n_req, T = kAttnWarps * 32;
@@ -705,7 +810,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) k_attn_split(const AttnParams
             const Req q = attn_req(p, r);
             for (int rt = 0; rt < p.tiles; ++rt) {
                 int f, n;
-                tile_steps(p, q, rt, f, n);
+                tile_steps<8>(p, q, rt, f, n);
                 sum += (int64_t) n * p.c.H;
             }
         }
@@ -719,13 +824,18 @@ __global__ void __launch_bounds__(kAttnWarps * 32) k_attn_split(const AttnParams
         __syncthreads();
         int64_t x = v - sum;
         for (int w = 0; w < warp; ++w) x += wsum[w];
-        for (int r = r0; r < r1; ++r) {
-            pre[r] = x;
-            const Req q = attn_req(p, r);
-            for (int rt = 0; rt < p.tiles; ++rt) {
-                int f, n;
-                tile_steps(p, q, rt, f, n);
-                x += (int64_t) n * p.c.H;
+        if (per == 1) {
+            if (r0 < r1) pre[r0] = x;
+            x += sum;
+        } else {
+            for (int r = r0; r < r1; ++r) {
+                pre[r] = x;
+                const Req q = attn_req(p, r);
+                for (int rt = 0; rt < p.tiles; ++rt) {
+                    int f, n;
+                    tile_steps<8>(p, q, rt, f, n);
+                    x += (int64_t) n * p.c.H;
+                }
             }
         }
         if (tid == T - 1) pre[R] = x;
@@ -733,8 +843,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32) k_attn_split(const AttnParams
     }
     if (blockIdx.x == 0)
         for (int r = tid; r <= R; r += T) p.pre[r] = pre[r];
+    asm volatile("griddepcontrol.launch_dependents;");
     const int64_t total = pre[R];
-    const int64_t per_cta = max((int64_t) (2 * kAttnWarps), (total + gridDim.x - 1) / gridDim.x);
+    const int64_t per_cta = max((int64_t) kAttnWarps, (total + gridDim.x - 1) / gridDim.x);
     const int64_t begin = (int64_t) blockIdx.x * per_cta, end = min(begin + per_cta, total);
     if (begin >= end) return;
     int r = 0;
@@ -755,146 +866,189 @@ __global__ void __launch_bounds__(kAttnWarps * 32) k_attn_split(const AttnParams
         int64_t in = (at - pre[r]) - (int64_t) h * all;
         int rt = 0, first = 0, n = 0;
         for (;; ++rt) {
-            tile_steps(p, q, rt, first, n);
+            tile_steps<8>(p, q, rt, first, n);
             if (in < n) break;
             in -= n;
         }
         const int64_t seg = at - in;                              // where the segment starts
         const int take = (int) min((int64_t) n - in, end - at);
-        stage_rows<D, SP>(p, q, h, rt, qf, rowf, warp, kAttnWarps, lane);
+        Walk<D, SP, 1> walk(p, smem_u32(rings + warp * Ring<D>::kBytes), r, h, first + (int) in, take, warp, kAttnWarps, lane);
+        stage_rows<D, 1>(p, q, h, rt, qf, rowf, warp, kAttnWarps, lane);
         __syncthreads();
-        Rows<D> rows;
+        Rows<D, 1> rows;
         rows.clear();
-        attend<D, SP>(p, qf, rowf, q, r, h, rt, first + (int) in, take, warp, kAttnWarps, rows, lane);
-        const int g = lane >> 2, qd = lane & 3;
+        walk.run(q, rt, qf, rowf, rows);
+        const int g = lane >> 2, qd = lane & 3, n_rows = q.n * p.G;
+        __syncthreads();                                          // the rings are free
 #pragma unroll
-        for (int half_w = kAttnWarps / 2; half_w; half_w /= 2) {
-            if (warp >= half_w && warp < 2 * half_w) {
-                float* b = mrg + (warp - half_w) * 16 * D;
+        for (int j = 0; j < D / 16; ++j) mrg[(warp * (D / 16) + j) * 32 + lane] = rows.o[0][j];
+        if (g == 0) {
 #pragma unroll
-                for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) b[(j * 4 + e) * 32 + lane] = rows.o[j][e];
-                if (qd == 0) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        ml[(warp - half_w) * 32 + g + 8 * i] = rows.m[i];
-                        ml[(warp - half_w) * 32 + 16 + g + 8 * i] = rows.l[i];
-                    }
-                }
-            }
-            __syncthreads();
-            if (warp < half_w) {
-                const float* b = mrg + warp * 16 * D;
-                float fa[2], fb[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float mb = ml[warp * 32 + g + 8 * i], lb = ml[warp * 32 + 16 + g + 8 * i];
-                    const float m = fmaxf(rows.m[i], mb);
-                    fa[i] = rows.m[i] == -INFINITY ? 0.0f : ex2(rows.m[i] - m);
-                    fb[i] = mb == -INFINITY ? 0.0f : ex2(mb - m);
-                    rows.m[i] = m;
-                    rows.l[i] = rows.l[i] * fa[i] + lb * fb[i];
-                }
-#pragma unroll
-                for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        rows.o[j][e] = rows.o[j][e] * fa[e >> 1] + b[(j * 4 + e) * 32 + lane] * fb[e >> 1];
-            }
-            __syncthreads();
+            for (int i = 0; i < 2; ++i) ml[warp * 16 + 2 * qd + i] = rows.m[0][i], ml[warp * 16 + 8 + 2 * qd + i] = rows.l[0][i];
         }
-        if (warp == 0) {
+        __syncthreads();
+        // warp w joins the four warps' tiles w D / 64 .. (w + 1) D / 64
+        constexpr int JT = D / 16 / kAttnWarps;
+        const int64_t slot = 2 * (int64_t) blockIdx.x + (seg > begin ? 1 : 0);
+        float m[2], l[2] = {0.0f, 0.0f}, f[2][kAttnWarps], x[2][2 * JT];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = 2 * qd + i;
+            m[i] = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kAttnWarps; ++w) m[i] = fmaxf(m[i], ml[w * 16 + row]);
+#pragma unroll
+            for (int w = 0; w < kAttnWarps; ++w) {
+                const float mw = ml[w * 16 + row];
+                f[i][w] = mw == -INFINITY ? 0.0f : ex2(mw - m[i]);
+                l[i] = fmaf(ml[w * 16 + 8 + row], f[i][w], l[i]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < JT; ++j) {
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kAttnWarps; ++w) {
+                const float4 v = mrg[(w * (D / 16) + warp * JT + j) * 32 + lane];
+                o.x = fmaf(v.x, f[0][w], o.x), o.y = fmaf(v.y, f[1][w], o.y);
+                o.z = fmaf(v.z, f[0][w], o.z), o.w = fmaf(v.w, f[1][w], o.w);
+            }
+            x[0][2 * j] = o.x, x[1][2 * j] = o.y, x[0][2 * j + 1] = o.z, x[1][2 * j + 1] = o.w;
+        }
+        const int col = Rows<D, 1>::column(warp * JT, g);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = 2 * qd + i, all_row = rt * 8 + row;
+            if (all_row >= n_rows) continue;
             if (take == n) {
-                write_rows<D>(p, q, h, rt, rows, lane);
+                const float inv = l[i] > 0.0f ? 1.0f / l[i] : 0.0f;     // a row that sees no key is zero
+                const int64_t to = (int64_t) (q.tok + all_row / p.G) * p.o_tok + (int64_t) (h * p.G + all_row % p.G) * p.o_head;
+#pragma unroll
+                for (int j = 0; j < 2 * JT; ++j) x[i][j] *= inv;
+                store_row<2 * JT>(p.o, to + col, p.type, x[i], p.wide_out);
             } else {
-                const int64_t slot = 2 * (int64_t) blockIdx.x + (seg > begin ? 1 : 0);
-                float* b = p.part + slot * 16 * D;
-                float* s = p.part + 2 * (int64_t) p.n_cta * 16 * D + slot * 32;
+                float* to = p.part + (slot * 8 + row) * D + col;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-#pragma unroll
-                    for (int half = 0; half < 2; ++half)
-#pragma unroll
-                        for (int j = 0; j < D / 8; j += 4)
-                            *(float4*) (b + (g + 8 * i) * D + out_col<D>(j, half, qd)) =
-                                make_float4(rows.o[j][2 * i + half], rows.o[j + 1][2 * i + half], rows.o[j + 2][2 * i + half],
-                                            rows.o[j + 3][2 * i + half]);
-                    if (qd == 0) s[g + 8 * i] = rows.m[i], s[16 + g + 8 * i] = rows.l[i];
+                for (int j = 0; j < 2 * JT; j += 2) *(float2*) (to + j) = make_float2(x[i][j], x[i][j + 1]);
+                if (warp == 0 && g == 0) {
+                    float* st = p.part + 2 * (int64_t) p.n_cta * 8 * D + slot * 16;
+                    st[row] = m[i], st[8 + row] = l[i];
                 }
             }
         }
+        __syncthreads();                                          // the rows are joined
         at += take;
     }
 }
 
-// One warp per (request, head, tile) row: the rows of the ranges that a segment was cut into, joined by their maxima;
-// zeros for a row of a segment without keys.  Segments inside one range were finished by k_attn_split.
+// CTA (segment, row): the parts of a row of a segment that was cut, joined by their maxima, eight warps taking parts in
+// turn; zeros for a row of a segment without keys.  Segments inside one range were finished by k_attn_split.
 template <int D>
-__global__ void __launch_bounds__(128) k_attn_join(const AttnParams p) {
-    const int lane = threadIdx.x & 31;
-    const int seg_id = blockIdx.x, i = blockIdx.y * 4 + (threadIdx.x >> 5);
+__global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ AttnParams p) {
+    constexpr int V = D / 32;
+    __shared__ float acc[8][D], stat[8][2];
+    asm volatile("griddepcontrol.wait;" ::: "memory");       // every CTA: the split is complete from here on
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int seg_id = blockIdx.x, i = blockIdx.y;
     const int rt = seg_id % p.tiles, h = seg_id / p.tiles % p.c.H, r = seg_id / p.tiles / p.c.H;
     const Req q = attn_req(p, r);
-    const int row = rt * 16 + i;
+    const int row = rt * 8 + i;
     if (row >= q.n * p.G) return;
     int first, n;
-    const int64_t total = p.pre[p.n_req];
-    const int64_t per_cta = max((int64_t) (2 * kAttnWarps), (total + p.n_cta - 1) / p.n_cta);
-    int64_t seg = p.pre[r] + (p.pre[r + 1] - p.pre[r]) / p.c.H * h;
+    const int64_t total = p.pre[p.n_req], p0 = p.pre[r], p1 = p.pre[r + 1];
+    const int64_t per_cta = max((int64_t) kAttnWarps, (total + p.n_cta - 1) / p.n_cta);
+    int64_t seg = p0 + (p1 - p0) / p.c.H * h;
     for (int t = 0; t < rt; ++t) {
-        tile_steps(p, q, t, first, n);
+        tile_steps<8>(p, q, t, first, n);
         seg += n;
     }
-    tile_steps(p, q, rt, first, n);
+    tile_steps<8>(p, q, rt, first, n);
     const int64_t out = (int64_t) (q.tok + row / p.G) * p.o_tok + (int64_t) (h * p.G + row % p.G) * p.o_head;
     if (n == 0) {
-        for (int d = lane; d < D; d += 32) store_elem(p.o, out + d, p.type, 0.0f);
+        for (int d = threadIdx.x; d < D; d += 256) store_elem(p.o, out + d, p.type, 0.0f);
         return;
     }
-    const int64_t c0 = seg / per_cta, c1 = (seg + n - 1) / per_cta;
+    const int c0 = (int) (seg / per_cta), c1 = (int) ((seg + n - 1) / per_cta);
     if (c0 == c1) return;
-    const float* stats = p.part + 2 * (int64_t) p.n_cta * 16 * D;
-    auto slot = [&](int64_t c) { return 2 * c + (seg > c * per_cta ? 1 : 0); };
+    const float* stats = p.part + 2 * (int64_t) p.n_cta * 8 * D;
+    auto slot = [&](int c) { return 2 * c + (seg > c * per_cta ? 1 : 0); };
     float m = -INFINITY;
-    for (int64_t c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, stats[slot(c) * 32 + i]);
+    for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, stats[slot(c) * 16 + i]);
     m = warp_max(m);
-    float acc[D / 32], l = 0.0f;
+    float a[V], l = 0.0f;
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j) acc[j] = 0.0f;
+    for (int j = 0; j < V; ++j) a[j] = 0.0f;
 #pragma unroll 4
-    for (int64_t c = c0; c <= c1; ++c) {
-        const float mc = stats[slot(c) * 32 + i], lc = stats[slot(c) * 32 + 16 + i];
+    for (int c = c0 + warp; c <= c1; c += 8) {
+        const int sl = slot(c);
+        const float mc = stats[sl * 16 + i], lc = stats[sl * 16 + 8 + i];
         const float f = mc == -INFINITY ? 0.0f : ex2(mc - m);
-        const float* b = p.part + (slot(c) * 16 + i) * D;
+        const float* b = p.part + ((int64_t) sl * 8 + i) * D;
         l = fmaf(lc, f, l);
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) acc[j] = fmaf(b[j * 32 + lane], f, acc[j]);
+        for (int j = 0; j < V; ++j) a[j] = fmaf(b[j * 32 + lane], f, a[j]);
     }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j) store_elem(p.o, out + j * 32 + lane, p.type, acc[j] * inv);
+    for (int j = 0; j < V; ++j) acc[warp][j * 32 + lane] = a[j];
+    if (lane == 0) stat[warp][0] = l;
+    __syncthreads();
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) l += stat[w][0];
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    for (int d = threadIdx.x; d < D; d += 256) {
+        float o = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) o += acc[w][d];
+        store_elem(p.o, out + d, p.type, o * inv);
+    }
 }
 
-// Many rows: one warp per 16-row tile, every step of the tile by the same warp; the four warps of a CTA take
-// neighbouring tiles of a head, so they share the codes through the caches.
+// Many rows: one warp per tile of 32 rows (head_dim 256: 16), every step of the tile by the same warp, which turns a
+// step's codes into operands once for all of them; the four warps of a CTA take neighbouring tiles of a head, so they share
+// the codes through the caches.
+template <int D>
+constexpr int kTileGroups = D == 256 ? 2 : 4;
 template <int D, int SP>
-__global__ void __launch_bounds__(kAttnWarps * 32) k_attn_tiles(const AttnParams p) {
-    extern __shared__ __align__(16) uint8_t smem[];
+__global__ void __launch_bounds__(kAttnWarps * 32) k_attn_tiles(const __grid_constant__ AttnParams p) {
+    constexpr int NB = kTileGroups<D>, TR = 8 * NB;
+    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr int kQ = NB * 3 * (D / 32) * 256;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint4* qf = (uint4*) smem + warp * SP * (D / 16) * 32;
-    float* rowf = (float*) ((uint4*) smem + kAttnWarps * SP * (D / 16) * 32) + warp * 16;
+    uint8_t* ring = smem + warp * (Ring<D>::kBytes + kQ + 128);
+    uint8_t* qf = ring + Ring<D>::kBytes;
+    float* rowf = (float*) (qf + kQ);
     const int rt = (gridDim.x - 1 - blockIdx.x) * kAttnWarps + warp, h = blockIdx.y, r = blockIdx.z;
     const Req q = attn_req(p, r);
-    if (rt * 16 >= q.n * p.G) return;
-    stage_rows<D, SP>(p, q, h, rt, qf, rowf, 0, 1, lane);
-    __syncwarp();
+    if (rt * TR >= q.n * p.G) return;
     int first, n;
-    tile_steps(p, q, rt, first, n);
-    Rows<D> rows;
+    tile_steps<TR>(p, q, rt, first, n);
+    Walk<D, SP, NB> walk(p, smem_u32(ring), r, h, first, n, 0, 1, lane);
+    stage_rows<D, NB>(p, q, h, rt, qf, rowf, 0, 1, lane);
+    __syncwarp();
+    Rows<D, NB> rows;
     rows.clear();
-    attend<D, SP>(p, qf, rowf, q, r, h, rt, first, n, 0, 1, rows, lane);
-    write_rows<D>(p, q, h, rt, rows, lane);
+    walk.run(q, rt, qf, rowf, rows);
+    const int g = lane >> 2, qd = lane & 3, n_rows = q.n * p.G;
+#pragma unroll
+    for (int u = 0; u < NB; ++u)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = rt * TR + u * 8 + 2 * qd + i;
+            if (row >= n_rows) continue;
+            const float inv = rows.l[u][i] > 0.0f ? 1.0f / rows.l[u][i] : 0.0f;
+            const int64_t to = (int64_t) (q.tok + row / p.G) * p.o_tok + (int64_t) (h * p.G + row % p.G) * p.o_head;
+#pragma unroll
+            for (int j0 = 0; j0 < D / 16; j0 += 4) {
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float4 o = rows.o[u][j0 + j];
+                    x[2 * j] = (i ? o.y : o.x) * inv, x[2 * j + 1] = (i ? o.w : o.z) * inv;
+                }
+                store_row<8>(p.o, to + Rows<D, NB>::column(j0, g), p.type, x, p.wide_out);
+            }
+        }
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -934,27 +1088,38 @@ int attn_plan(const tsb_kv8* c, const tsb_kv8_attn* d, AttnPlan& a) {
     a.G = d->q_heads / c->n_kv_heads;
     const int64_t rows = (int64_t) d->max_q * a.G;
     if (rows > (1 << 28)) return cfail(TSB_ERR_UNSUPPORTED, "kv8_attention: too many query rows");
-    a.tiles = (int) ((rows + 15) / 16);
     a.split = rows <= kSplitRows;
+    const int tile = a.split ? 8 : c->head_dim == 256 ? 8 * kTileGroups<256> : 8 * kTileGroups<128>;
+    a.tiles = (int) ((rows + tile - 1) / tile);
     const int sms = sm_count();
     if (!sms) return cfail(TSB_ERR_CUDA, "kv8_attention: no CUDA device");
-    a.n_cta = sms * (c->head_dim == 256 ? 2 : c->head_dim == 128 ? 3 : 4);
-    a.ws = a.split ? (((uint64_t) d->n_req + 1) * 8 + 255) / 256 * 256 + (uint64_t) a.n_cta * 2 * (16 * c->head_dim + 32) * 4 : 0;
+    a.n_cta = sms * (c->head_dim == 256 ? kSplitCtas<256> : c->head_dim == 128 ? kSplitCtas<128> : kSplitCtas<64>);
+    a.ws = a.split ? (((uint64_t) d->n_req + 1) * 8 + 255) / 256 * 256 + (uint64_t) a.n_cta * 2 * (8 * c->head_dim + 16) * 4 : 0;
     return TSB_OK;
 }
 
 template <int D, int SP>
-int launch_attn(const AttnParams& p, const AttnPlan& a, cudaStream_t st) {
-    const int qf = SP * (D / 16) * 32 * 16;
+int launch_attn(const AttnParams& p, const AttnPlan& a, int rows, cudaStream_t st) {
     if (a.split) {
-        const int sm = qf + 2 * 16 * D * 4 + 64 * 4 + 16 * 4 + (p.n_req + 1) * 8;
+        const int sm = kAttnWarps * Ring<D>::kBytes + 3 * (D / 32) * 256 + kAttnWarps * 64 + 32 + (p.n_req + 1) * 8;
         if (sm > 48 * 1024 &&
             cudaFuncSetAttribute(k_attn_split<D, SP>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm) != cudaSuccess)
             return ccuda("kv8_attention: shared memory");
         k_attn_split<D, SP><<<a.n_cta, kAttnWarps * 32, sm, st>>>(p);
-        k_attn_join<D><<<dim3((unsigned) (p.n_req * p.c.H * p.tiles), 4), 128, 0, st>>>(p);
+        if (int rc = ccuda("kv8_attention")) return rc;
+        // the join's CTAs come up while the split runs; each waits for it (griddepcontrol.wait) before it reads
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned) (p.n_req * p.c.H * p.tiles), (unsigned) std::min(rows, 8));
+        cfg.blockDim = dim3(256);
+        cfg.stream = st;
+        cudaLaunchAttribute at{};
+        at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+        cudaLaunchKernelEx(&cfg, k_attn_join<D>, p);
     } else {
-        const int sm = kAttnWarps * (qf + 64);
+        const int sm = kAttnWarps * (kTileGroups<D> * 3 * (D / 32) * 256 + 128 + Ring<D>::kBytes);
         if (sm > 48 * 1024 &&
             cudaFuncSetAttribute(k_attn_tiles<D, SP>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm) != cudaSuccess)
             return ccuda("kv8_attention: shared memory");
@@ -1058,12 +1223,14 @@ int tsb_kv8_attention(const tsb_kv8* cache, const tsb_kv8_attn* d, const void* q
     p.tiles = a.tiles, p.n_cta = a.n_cta;
     p.pre = (int64_t*) workspace;
     p.part = (float*) ((uint8_t*) workspace + (((uint64_t) d->n_req + 1) * 8 + 255) / 256 * 256);
+    p.wide_out = !((uintptr_t) out % 16 || (d->o_tok * es) % 16 || (d->o_head * es) % 16);
+    const int rows = (int) std::min<int64_t>((int64_t) d->max_q * a.G, 1 << 20);
     const bool two = d->elem_type == E_F32;
     cudaStream_t st = cst(stream);
     switch (cache->head_dim) {
-        case 64: return two ? launch_attn<64, 2>(p, a, st) : launch_attn<64, 1>(p, a, st);
-        case 128: return two ? launch_attn<128, 2>(p, a, st) : launch_attn<128, 1>(p, a, st);
-        default: return two ? launch_attn<256, 2>(p, a, st) : launch_attn<256, 1>(p, a, st);
+        case 64: return two ? launch_attn<64, 2>(p, a, rows, st) : launch_attn<64, 1>(p, a, rows, st);
+        case 128: return two ? launch_attn<128, 2>(p, a, rows, st) : launch_attn<128, 1>(p, a, rows, st);
+        default: return two ? launch_attn<256, 2>(p, a, rows, st) : launch_attn<256, 1>(p, a, rows, st);
     }
 }
 
