@@ -9,6 +9,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdint>
@@ -39,13 +40,39 @@ int ccuda(const char* what) {
 }
 cudaStream_t cst(void* s) { return (cudaStream_t) s; }
 
-int sm_count() {
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+constexpr int kMaxDev = 64;
+int device() {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDev) {
         cudaGetLastError();
-        return 0;
+        return -1;
+    }
+    return dev;
+}
+int sm_count() {
+    static std::atomic<int> known[kMaxDev];
+    const int dev = device();
+    if (dev < 0) return 0;
+    int n = known[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+            cudaGetLastError();
+            return 0;
+        }
+        known[dev].store(n, std::memory_order_relaxed);
     }
     return n;
+}
+// A kernel's dynamic shared memory above 48 KB, granted once a device: `most` is the largest asked for so far.
+template <class K>
+bool allow_smem(K* kernel, std::atomic<int> (&most)[kMaxDev], int bytes) {
+    if (bytes <= 48 * 1024) return true;
+    const int dev = device();
+    if (dev < 0) return false;
+    if (most[dev].load(std::memory_order_relaxed) >= bytes) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    most[dev].store(bytes, std::memory_order_relaxed);
+    return true;
 }
 
 // ------------------------------------------------------------------------------------------------ block tables
@@ -350,7 +377,7 @@ struct AttnParams {
     int tiles;                       // row tiles of the longest request
     // split over CTAs: steps before each request, partial rows
     int64_t* pre;                    // [n_req + 1]
-    float* part;                     // [2 * CTAs][8][D], then their maxima and sums [2 * CTAs][2][8]
+    float* part;                     // [2 * CTAs][tile rows][D], then their maxima and sums [2 * CTAs][2][tile rows]
     int n_cta;
     bool wide_out;                   // 16-byte aligned output rows
 };
@@ -382,6 +409,16 @@ __device__ __forceinline__ void tile_steps(const AttnParams& p, const Req& q, in
     if (hi <= 0) return;
     first = lo / kStep;
     n = (hi + kStep - 1) / kStep - first;
+}
+
+// What a step of a tile costs the split, in units: measured per step, a tile of up to 8 rows to one of 9 to 16.
+constexpr int kLight = 3, kHeavy = 4;
+template <int TR>
+__device__ __forceinline__ int step_cost(const AttnParams& p, const Req& q, int rt) {
+    return q.n * p.G - rt * TR > 8 ? kHeavy : kLight;
+}
+__device__ __forceinline__ int64_t units_per_cta(int64_t total, int ctas) {
+    return max((int64_t) kAttnWarps * kHeavy, (total + ctas - 1) / ctas);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -544,7 +581,7 @@ __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 
 //   fp16 value (11 bits down to 2^-29 of the largest weight; 2^-40 of it below) and o accumulates in the tensor cores.
 // SP 2, fp32 outputs: weights as two fp16 values; a step's product starts from zero and is added in fp32 times the value
 //   scale, since the tensor cores' sums truncate.
-template <int D, int SP, int NB>
+template <int D, int SP>
 struct Walk {
     const AttnParams& p;
     const int32_t* tab;
@@ -585,8 +622,9 @@ struct Walk {
         stage_copy = stage_copy + 1 == Ring<D>::kDepth ? 0 : stage_copy + 1;
     }
 
-    __device__ __forceinline__ void run(const Req& q, int rt, const uint8_t* qf, const float* rowf, Rows<D, NB>& R) {
-        constexpr int TR = 8 * NB;
+    // tile rt of TR rows, its first NB groups
+    template <int TR, int NB, int NBR>
+    __device__ __forceinline__ void run(const Req& q, int rt, const uint8_t* qf, const float* rowf, Rows<D, NBR>& R) {
         const int g = lane >> 2, qd = lane & 3, rows = q.n * p.G;
         constexpr bool QREG = NB == 1 && D <= 128;       // the rows' operands stay in registers where they fit
         const uint2* qp = (const uint2*) qf + lane;
@@ -782,27 +820,30 @@ __device__ __forceinline__ void store_row(void* o, int64_t at, int type, const f
     }
 }
 
-template <int D>
-constexpr int kSplitCtas = D == 256 ? 3 : D == 128 ? 4 : 5;   // CTAs a SM holds
+// CTAs a SM holds, for tiles of 8 (NB 1) and of 16 rows (NB 2, where a request has more than 8: a step's codes are then
+// read and turned into operands once for both groups; tiles with up to 8 rows skip the second)
+template <int D, int NB>
+constexpr int kSplitCtas = NB == 1 ? (D == 256 ? 3 : D == 128 ? 4 : 5) : (D == 256 ? 2 : D == 128 ? 3 : 4);
 
-// The steps of all (request, head, tile of 8 rows) segments, one after the other (request, then head, then tile), are cut into
+// The steps of all (request, head, tile) segments, one after the other (request, then head, then tile), are cut into
 // equal ranges, one per CTA; a range's warps take its steps in turn and join their rows through shared memory at the
 // end of each segment.  A segment inside one range is finished there; one cut by a range's end leaves its rows, maxima
 // and sums for k_attn_join.  So a lone request of 131,072 tokens and 64 requests of uneven lengths fill the GPU alike.
-template <int D, int SP>
-__global__ void __launch_bounds__(kAttnWarps * 32, kSplitCtas<D>) k_attn_split(const __grid_constant__ AttnParams p) {
+template <int D, int SP, int NB>
+__global__ void __launch_bounds__(kAttnWarps * 32, kSplitCtas<D, NB>) k_attn_split(const __grid_constant__ AttnParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
-    uint8_t* rings = smem;                                             // [warps] rings; then [warps][8][D] rows to join
+    uint8_t* rings = smem;                                             // [warps] rings; then [warps][8 NB][D] rows to join
+    constexpr int TR = 8 * NB;
     float4* mrg = (float4*) rings;
-    uint8_t* qf = rings + kAttnWarps * Ring<D>::kBytes;                // [3][D / 32][32][8]
-    float* ml = (float*) (qf + 3 * (D / 32) * 256);                    // [warps][2][8]
-    float* rowf = ml + kAttnWarps * 16;                                // [8]
-    int64_t* pre = (int64_t*) (rowf + 8);                              // [n_req + 1]
-    static_assert(Ring<D>::kBytes >= 8 * D * 4, "the rows to join lie over the rings");
+    uint8_t* qf = rings + kAttnWarps * Ring<D>::kBytes;                // [NB][3][D / 32][32][8]
+    float* ml = (float*) (qf + NB * 3 * (D / 32) * 256);               // [warps][2][TR]
+    float* rowf = ml + kAttnWarps * 2 * TR;                            // [TR]
+    int64_t* pre = (int64_t*) (rowf + TR);                             // [n_req + 1]
+    static_assert(Ring<D>::kBytes >= TR * D * 4, "the rows to join lie over the rings");
     __shared__ int64_t wsum[kAttnWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int R = p.n_req, T = kAttnWarps * 32;
-    // steps before each request
+    // units before each request
     {
         const int per = (R + T - 1) / T, r0 = min(tid * per, R), r1 = min(r0 + per, R);
         int64_t sum = 0;
@@ -810,8 +851,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kSplitCtas<D>) k_attn_split(c
             const Req q = attn_req(p, r);
             for (int rt = 0; rt < p.tiles; ++rt) {
                 int f, n;
-                tile_steps<8>(p, q, rt, f, n);
-                sum += (int64_t) n * p.c.H;
+                tile_steps<TR>(p, q, rt, f, n);
+                sum += (int64_t) n * p.c.H * step_cost<TR>(p, q, rt);
             }
         }
         int64_t v = sum;
@@ -833,8 +874,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kSplitCtas<D>) k_attn_split(c
                 const Req q = attn_req(p, r);
                 for (int rt = 0; rt < p.tiles; ++rt) {
                     int f, n;
-                    tile_steps<8>(p, q, rt, f, n);
-                    x += (int64_t) n * p.c.H;
+                    tile_steps<TR>(p, q, rt, f, n);
+                    x += (int64_t) n * p.c.H * step_cost<TR>(p, q, rt);
                 }
             }
         }
@@ -845,7 +886,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kSplitCtas<D>) k_attn_split(c
         for (int r = tid; r <= R; r += T) p.pre[r] = pre[r];
     asm volatile("griddepcontrol.launch_dependents;");
     const int64_t total = pre[R];
-    const int64_t per_cta = max((int64_t) kAttnWarps, (total + gridDim.x - 1) / gridDim.x);
+    const int64_t per_cta = units_per_cta(total, gridDim.x);
     const int64_t begin = (int64_t) blockIdx.x * per_cta, end = min(begin + per_cta, total);
     if (begin >= end) return;
     int r = 0;
@@ -861,146 +902,182 @@ __global__ void __launch_bounds__(kAttnWarps * 32, kSplitCtas<D>) k_attn_split(c
     for (int64_t at = begin; at < end;) {
         while (pre[r + 1] <= at) ++r;
         const Req q = attn_req(p, r);
-        const int64_t all = (pre[r + 1] - pre[r]) / p.c.H;        // steps of one head
+        const int64_t all = (pre[r + 1] - pre[r]) / p.c.H;        // units of one head
         const int h = (int) ((at - pre[r]) / all);
         int64_t in = (at - pre[r]) - (int64_t) h * all;
-        int rt = 0, first = 0, n = 0;
+        int rt = 0, first = 0, n = 0, cost = kLight;
         for (;; ++rt) {
-            tile_steps<8>(p, q, rt, first, n);
-            if (in < n) break;
-            in -= n;
+            tile_steps<TR>(p, q, rt, first, n);
+            cost = step_cost<TR>(p, q, rt);
+            if (in < (int64_t) n * cost) break;
+            in -= (int64_t) n * cost;
         }
         const int64_t seg = at - in;                              // where the segment starts
-        const int take = (int) min((int64_t) n - in, end - at);
-        Walk<D, SP, 1> walk(p, smem_u32(rings + warp * Ring<D>::kBytes), r, h, first + (int) in, take, warp, kAttnWarps, lane);
-        stage_rows<D, 1>(p, q, h, rt, qf, rowf, warp, kAttnWarps, lane);
+        const int64_t stop = min((int64_t) n * cost, end - seg);
+        at = seg + stop;
+        const int s0 = (int) ((in + cost - 1) / cost), take = (int) ((stop + cost - 1) / cost) - s0;
+        if (take <= 0) continue;                                  // the range ends within a step: the next one's
+        Walk<D, SP> walk(p, smem_u32(rings + warp * Ring<D>::kBytes), r, h, first + s0, take, warp, kAttnWarps, lane);
+        stage_rows<D, NB>(p, q, h, rt, qf, rowf, warp, kAttnWarps, lane);
         __syncthreads();
-        Rows<D, 1> rows;
+        Rows<D, NB> rows;
         rows.clear();
-        walk.run(q, rt, qf, rowf, rows);
-        const int g = lane >> 2, qd = lane & 3, n_rows = q.n * p.G;
+        const int n_rows = q.n * p.G;
+        if (NB == 1 || n_rows - rt * TR > 8) walk.template run<TR, NB>(q, rt, qf, rowf, rows);
+        else walk.template run<TR, 1>(q, rt, qf, rowf, rows);
+        const int g = lane >> 2, qd = lane & 3;
         __syncthreads();                                          // the rings are free
 #pragma unroll
-        for (int j = 0; j < D / 16; ++j) mrg[(warp * (D / 16) + j) * 32 + lane] = rows.o[0][j];
-        if (g == 0) {
+        for (int u = 0; u < NB; ++u) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) ml[warp * 16 + 2 * qd + i] = rows.m[0][i], ml[warp * 16 + 8 + 2 * qd + i] = rows.l[0][i];
+            for (int j = 0; j < D / 16; ++j) mrg[((warp * NB + u) * (D / 16) + j) * 32 + lane] = rows.o[u][j];
+            if (g == 0) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    ml[warp * 2 * TR + u * 8 + 2 * qd + i] = rows.m[u][i];
+                    ml[warp * 2 * TR + TR + u * 8 + 2 * qd + i] = rows.l[u][i];
+                }
+            }
         }
         __syncthreads();
         // warp w joins the four warps' tiles w D / 64 .. (w + 1) D / 64
         constexpr int JT = D / 16 / kAttnWarps;
         const int64_t slot = 2 * (int64_t) blockIdx.x + (seg > begin ? 1 : 0);
-        float m[2], l[2] = {0.0f, 0.0f}, f[2][kAttnWarps], x[2][2 * JT];
+        const int col = Rows<D, NB>::column(warp * JT, g);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int row = 2 * qd + i;
-            m[i] = -INFINITY;
+        for (int u = 0; u < NB; ++u) {
+            if (rt * TR + u * 8 >= n_rows) continue;
+            float m[2], l[2] = {0.0f, 0.0f}, f[2][kAttnWarps], x[2][2 * JT];
 #pragma unroll
-            for (int w = 0; w < kAttnWarps; ++w) m[i] = fmaxf(m[i], ml[w * 16 + row]);
+            for (int i = 0; i < 2; ++i) {
+                const float* st = ml + u * 8 + 2 * qd + i;
+                m[i] = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < kAttnWarps; ++w) {
-                const float mw = ml[w * 16 + row];
-                f[i][w] = mw == -INFINITY ? 0.0f : ex2(mw - m[i]);
-                l[i] = fmaf(ml[w * 16 + 8 + row], f[i][w], l[i]);
+                for (int w = 0; w < kAttnWarps; ++w) m[i] = fmaxf(m[i], st[w * 2 * TR]);
+#pragma unroll
+                for (int w = 0; w < kAttnWarps; ++w) {
+                    const float mw = st[w * 2 * TR];
+                    f[i][w] = mw == -INFINITY ? 0.0f : ex2(mw - m[i]);
+                    l[i] = fmaf(st[w * 2 * TR + TR], f[i][w], l[i]);
+                }
             }
-        }
 #pragma unroll
-        for (int j = 0; j < JT; ++j) {
-            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int j = 0; j < JT; ++j) {
+                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int w = 0; w < kAttnWarps; ++w) {
-                const float4 v = mrg[(w * (D / 16) + warp * JT + j) * 32 + lane];
-                o.x = fmaf(v.x, f[0][w], o.x), o.y = fmaf(v.y, f[1][w], o.y);
-                o.z = fmaf(v.z, f[0][w], o.z), o.w = fmaf(v.w, f[1][w], o.w);
+                for (int w = 0; w < kAttnWarps; ++w) {
+                    const float4 v = mrg[((w * NB + u) * (D / 16) + warp * JT + j) * 32 + lane];
+                    o.x = fmaf(v.x, f[0][w], o.x), o.y = fmaf(v.y, f[1][w], o.y);
+                    o.z = fmaf(v.z, f[0][w], o.z), o.w = fmaf(v.w, f[1][w], o.w);
+                }
+                x[0][2 * j] = o.x, x[1][2 * j] = o.y, x[0][2 * j + 1] = o.z, x[1][2 * j + 1] = o.w;
             }
-            x[0][2 * j] = o.x, x[1][2 * j] = o.y, x[0][2 * j + 1] = o.z, x[1][2 * j + 1] = o.w;
-        }
-        const int col = Rows<D, 1>::column(warp * JT, g);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int row = 2 * qd + i, all_row = rt * 8 + row;
-            if (all_row >= n_rows) continue;
-            if (take == n) {
-                const float inv = l[i] > 0.0f ? 1.0f / l[i] : 0.0f;     // a row that sees no key is zero
-                const int64_t to = (int64_t) (q.tok + all_row / p.G) * p.o_tok + (int64_t) (h * p.G + all_row % p.G) * p.o_head;
+            for (int i = 0; i < 2; ++i) {
+                const int row = u * 8 + 2 * qd + i, all_row = rt * TR + row;
+                if (all_row >= n_rows) continue;
+                if (take == n) {
+                    const float inv = l[i] > 0.0f ? 1.0f / l[i] : 0.0f;     // a row that sees no key is zero
+                    const int64_t to = (int64_t) (q.tok + all_row / p.G) * p.o_tok + (int64_t) (h * p.G + all_row % p.G) * p.o_head;
 #pragma unroll
-                for (int j = 0; j < 2 * JT; ++j) x[i][j] *= inv;
-                store_row<2 * JT>(p.o, to + col, p.type, x[i], p.wide_out);
-            } else {
-                float* to = p.part + (slot * 8 + row) * D + col;
+                    for (int j = 0; j < 2 * JT; ++j) x[i][j] *= inv;
+                    store_row<2 * JT>(p.o, to + col, p.type, x[i], p.wide_out);
+                } else {
+                    float* to = p.part + (slot * TR + row) * D + col;
 #pragma unroll
-                for (int j = 0; j < 2 * JT; j += 2) *(float2*) (to + j) = make_float2(x[i][j], x[i][j + 1]);
-                if (warp == 0 && g == 0) {
-                    float* st = p.part + 2 * (int64_t) p.n_cta * 8 * D + slot * 16;
-                    st[row] = m[i], st[8 + row] = l[i];
+                    for (int j = 0; j < 2 * JT; j += 2) *(float2*) (to + j) = make_float2(x[i][j], x[i][j + 1]);
+                    if (warp == 0 && g == 0) {
+                        float* st = p.part + 2 * (int64_t) p.n_cta * TR * D + slot * 2 * TR;
+                        st[row] = m[i], st[TR + row] = l[i];
+                    }
                 }
             }
         }
         __syncthreads();                                          // the rows are joined
-        at += take;
     }
 }
 
-// CTA (segment, row): the parts of a row of a segment that was cut, joined by their maxima, eight warps taking parts in
-// turn; zeros for a row of a segment without keys.  Segments inside one range were finished by k_attn_split.
-template <int D>
+// CTA (segment, share): the parts of the rows of a segment that was cut, joined by their maxima, row and 64 columns at a time:
+// a warp an item when the parts are few, all eight warps on one item, parts in turn, when they are many (a long request).
+// Zeros for the rows of a segment without keys.  Segments inside one range were finished by k_attn_split.  What the parts
+// do not decide is read before the wait for the split's end.
+template <int D, int TR>
 __global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ AttnParams p) {
-    constexpr int V = D / 32;
-    __shared__ float acc[8][D], stat[8][2];
-    asm volatile("griddepcontrol.wait;" ::: "memory");       // every CTA: the split is complete from here on
+    __shared__ float2 acc[8][32];
+    __shared__ float stat[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int seg_id = blockIdx.x, i = blockIdx.y;
+    const int seg_id = blockIdx.x;
     const int rt = seg_id % p.tiles, h = seg_id / p.tiles % p.c.H, r = seg_id / p.tiles / p.c.H;
     const Req q = attn_req(p, r);
-    const int row = rt * 8 + i;
-    if (row >= q.n * p.G) return;
     int first, n;
-    const int64_t total = p.pre[p.n_req], p0 = p.pre[r], p1 = p.pre[r + 1];
-    const int64_t per_cta = max((int64_t) kAttnWarps, (total + p.n_cta - 1) / p.n_cta);
-    int64_t seg = p0 + (p1 - p0) / p.c.H * h;
+    int64_t seg = 0;
     for (int t = 0; t < rt; ++t) {
-        tile_steps<8>(p, q, t, first, n);
-        seg += n;
+        tile_steps<TR>(p, q, t, first, n);
+        seg += (int64_t) n * step_cost<TR>(p, q, t);
     }
-    tile_steps<8>(p, q, rt, first, n);
-    const int64_t out = (int64_t) (q.tok + row / p.G) * p.o_tok + (int64_t) (h * p.G + row % p.G) * p.o_head;
-    if (n == 0) {
-        for (int d = threadIdx.x; d < D; d += 256) store_elem(p.o, out + d, p.type, 0.0f);
+    tile_steps<TR>(p, q, rt, first, n);
+    const int cost = step_cost<TR>(p, q, rt);
+    const int items = min(max(q.n * p.G - rt * TR, 0), TR) * (D / 64);
+    asm volatile("griddepcontrol.wait;" ::: "memory");       // every CTA: the split is complete from here on
+    if (items == 0) return;
+    const int64_t total = p.pre[p.n_req], p0 = p.pre[r], p1 = p.pre[r + 1], per_cta = units_per_cta(total, p.n_cta);
+    seg += p0 + (p1 - p0) / p.c.H * h;
+    const int c0 = (int) (seg / per_cta);
+    int c1 = n ? (int) ((seg + (int64_t) n * cost - 1) / per_cta) : c0;
+    if (n) {
+        if (((c0 + 1) * per_cta - seg + cost - 1) / cost >= n) return;                    // finished by the split
+        if ((c1 * per_cta - seg + cost - 1) / cost >= n) --c1;                            // its share was within a step
+    }
+    const float* stats = p.part + 2 * (int64_t) p.n_cta * TR * D;
+    auto slot = [&](int c) { return 2 * c + (seg > c * per_cta ? 1 : 0); };
+    auto join = [&](int i, int col, int from, int by, float2& a, float& l) {
+        float m = -INFINITY;
+        for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, stats[slot(c) * 2 * TR + i]);
+        m = warp_max(m);
+        a = make_float2(0.0f, 0.0f), l = 0.0f;
+#pragma unroll 8
+        for (int c = c0 + from; c <= c1; c += by) {
+            const int sl = slot(c);
+            const float mc = stats[sl * 2 * TR + i], lc = stats[sl * 2 * TR + TR + i];
+            const float2 b = *(const float2*) (p.part + ((int64_t) sl * TR + i) * D + col);
+            const float f = mc == -INFINITY ? 0.0f : ex2(mc - m);
+            l = fmaf(lc, f, l);
+            a.x = fmaf(b.x, f, a.x), a.y = fmaf(b.y, f, a.y);
+        }
+    };
+    auto write = [&](int i, int col, float2 a, float l) {
+        const int row = rt * TR + i;
+        const int64_t out = (int64_t) (q.tok + row / p.G) * p.o_tok + (int64_t) (h * p.G + row % p.G) * p.o_head + col;
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const float x[2] = {a.x * inv, a.y * inv};
+        store_row<2>(p.o, out, p.type, x, p.wide_out);
+    };
+    if (n == 0 || c1 - c0 < 16) {
+        for (int it = blockIdx.y * 8 + warp; it < items; it += gridDim.y * 8) {
+            const int i = it / (D / 64), col = it % (D / 64) * 64 + 2 * lane;
+            float2 a = make_float2(0.0f, 0.0f);
+            float l = 0.0f;
+            if (n) join(i, col, 0, 1, a, l);
+            write(i, col, a, l);
+        }
         return;
     }
-    const int c0 = (int) (seg / per_cta), c1 = (int) ((seg + n - 1) / per_cta);
-    if (c0 == c1) return;
-    const float* stats = p.part + 2 * (int64_t) p.n_cta * 8 * D;
-    auto slot = [&](int c) { return 2 * c + (seg > c * per_cta ? 1 : 0); };
-    float m = -INFINITY;
-    for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, stats[slot(c) * 16 + i]);
-    m = warp_max(m);
-    float a[V], l = 0.0f;
+    for (int it = blockIdx.y; it < items; it += gridDim.y) {
+        const int i = it / (D / 64), col = it % (D / 64) * 64 + 2 * lane;
+        float2 a;
+        float l;
+        join(i, col, warp, 8, a, l);
+        acc[warp][lane] = a;
+        if (lane == 0) stat[warp] = l;
+        __syncthreads();
+        if (warp == 0) {
+            l = 0.0f;
+            a = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int j = 0; j < V; ++j) a[j] = 0.0f;
-#pragma unroll 4
-    for (int c = c0 + warp; c <= c1; c += 8) {
-        const int sl = slot(c);
-        const float mc = stats[sl * 16 + i], lc = stats[sl * 16 + 8 + i];
-        const float f = mc == -INFINITY ? 0.0f : ex2(mc - m);
-        const float* b = p.part + ((int64_t) sl * 8 + i) * D;
-        l = fmaf(lc, f, l);
-#pragma unroll
-        for (int j = 0; j < V; ++j) a[j] = fmaf(b[j * 32 + lane], f, a[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j) acc[warp][j * 32 + lane] = a[j];
-    if (lane == 0) stat[warp][0] = l;
-    __syncthreads();
-    l = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) l += stat[w][0];
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    for (int d = threadIdx.x; d < D; d += 256) {
-        float o = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) o += acc[w][d];
-        store_elem(p.o, out + d, p.type, o * inv);
+            for (int w = 0; w < 8; ++w) l += stat[w], a.x += acc[w][lane].x, a.y += acc[w][lane].y;
+            write(i, col, a, l);
+        }
+        __syncthreads();
     }
 }
 
@@ -1023,12 +1100,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32) k_attn_tiles(const __grid_con
     if (rt * TR >= q.n * p.G) return;
     int first, n;
     tile_steps<TR>(p, q, rt, first, n);
-    Walk<D, SP, NB> walk(p, smem_u32(ring), r, h, first, n, 0, 1, lane);
+    Walk<D, SP> walk(p, smem_u32(ring), r, h, first, n, 0, 1, lane);
     stage_rows<D, NB>(p, q, h, rt, qf, rowf, 0, 1, lane);
     __syncwarp();
     Rows<D, NB> rows;
     rows.clear();
-    walk.run(q, rt, qf, rowf, rows);
+    walk.template run<TR, NB>(q, rt, qf, rowf, rows);
     const int g = lane >> 2, qd = lane & 3, n_rows = q.n * p.G;
 #pragma unroll
     for (int u = 0; u < NB; ++u)
@@ -1070,7 +1147,7 @@ Cache cache_of(const tsb_kv8* c) {
 bool elem_ok(int t) { return t == E_F32 || t == E_F16 || t == E_BF16; }
 
 struct AttnPlan {
-    int G, tiles, n_cta;
+    int G, tiles, n_cta, groups;
     bool split;
     uint64_t ws;
 };
@@ -1089,42 +1166,45 @@ int attn_plan(const tsb_kv8* c, const tsb_kv8_attn* d, AttnPlan& a) {
     const int64_t rows = (int64_t) d->max_q * a.G;
     if (rows > (1 << 28)) return cfail(TSB_ERR_UNSUPPORTED, "kv8_attention: too many query rows");
     a.split = rows <= kSplitRows;
-    const int tile = a.split ? 8 : c->head_dim == 256 ? 8 * kTileGroups<256> : 8 * kTileGroups<128>;
-    a.tiles = (int) ((rows + tile - 1) / tile);
+    a.groups = !a.split ? (c->head_dim == 256 ? kTileGroups<256> : kTileGroups<128>) : rows <= 8 ? 1 : 2;
+    a.tiles = (int) ((rows + 8 * a.groups - 1) / (8 * a.groups));
     const int sms = sm_count();
     if (!sms) return cfail(TSB_ERR_CUDA, "kv8_attention: no CUDA device");
-    a.n_cta = sms * (c->head_dim == 256 ? kSplitCtas<256> : c->head_dim == 128 ? kSplitCtas<128> : kSplitCtas<64>);
-    a.ws = a.split ? (((uint64_t) d->n_req + 1) * 8 + 255) / 256 * 256 + (uint64_t) a.n_cta * 2 * (8 * c->head_dim + 16) * 4 : 0;
+    const int d_ = c->head_dim;
+    a.n_cta = sms * (a.groups == 1 ? (d_ == 256 ? kSplitCtas<256, 1> : d_ == 128 ? kSplitCtas<128, 1> : kSplitCtas<64, 1>)
+                                   : (d_ == 256 ? kSplitCtas<256, 2> : d_ == 128 ? kSplitCtas<128, 2> : kSplitCtas<64, 2>));
+    a.ws = a.split ? (((uint64_t) d->n_req + 1) * 8 + 255) / 256 * 256 + (uint64_t) a.n_cta * 2 * 8 * a.groups * (c->head_dim + 2) * 4 : 0;
     return TSB_OK;
 }
 
+template <int D, int SP, int NB>
+int launch_split(const AttnParams& p, const AttnPlan& a, int rows, cudaStream_t st) {
+    static std::atomic<int> most[kMaxDev];
+    const int sm = kAttnWarps * Ring<D>::kBytes + NB * (3 * (D / 32) * 256 + kAttnWarps * 64 + 32) + (p.n_req + 1) * 8;
+    if (!allow_smem(k_attn_split<D, SP, NB>, most, sm)) return ccuda("kv8_attention: shared memory");
+    k_attn_split<D, SP, NB><<<a.n_cta, kAttnWarps * 32, sm, st>>>(p);
+    if (int rc = ccuda("kv8_attention")) return rc;
+    // the join's CTAs come up while the split runs; each waits for it (griddepcontrol.wait) before it reads its results
+    cudaLaunchConfig_t cfg{};
+    const int segs = p.n_req * p.c.H * p.tiles, items = std::min(rows, 8 * NB) * (D / 64);
+    cfg.gridDim = dim3((unsigned) segs, (unsigned) std::max(1, std::min(items, a.n_cta / segs)));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, k_attn_join<D, 8 * NB>, p);
+    return ccuda("kv8_attention: join");
+}
 template <int D, int SP>
 int launch_attn(const AttnParams& p, const AttnPlan& a, int rows, cudaStream_t st) {
-    if (a.split) {
-        const int sm = kAttnWarps * Ring<D>::kBytes + 3 * (D / 32) * 256 + kAttnWarps * 64 + 32 + (p.n_req + 1) * 8;
-        if (sm > 48 * 1024 &&
-            cudaFuncSetAttribute(k_attn_split<D, SP>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm) != cudaSuccess)
-            return ccuda("kv8_attention: shared memory");
-        k_attn_split<D, SP><<<a.n_cta, kAttnWarps * 32, sm, st>>>(p);
-        if (int rc = ccuda("kv8_attention")) return rc;
-        // the join's CTAs come up while the split runs; each waits for it (griddepcontrol.wait) before it reads
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned) (p.n_req * p.c.H * p.tiles), (unsigned) std::min(rows, 8));
-        cfg.blockDim = dim3(256);
-        cfg.stream = st;
-        cudaLaunchAttribute at{};
-        at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        at.val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = &at;
-        cfg.numAttrs = 1;
-        cudaLaunchKernelEx(&cfg, k_attn_join<D>, p);
-    } else {
-        const int sm = kAttnWarps * (kTileGroups<D> * 3 * (D / 32) * 256 + 128 + Ring<D>::kBytes);
-        if (sm > 48 * 1024 &&
-            cudaFuncSetAttribute(k_attn_tiles<D, SP>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm) != cudaSuccess)
-            return ccuda("kv8_attention: shared memory");
-        k_attn_tiles<D, SP><<<dim3((unsigned) ((p.tiles + kAttnWarps - 1) / kAttnWarps), p.c.H, p.n_req), kAttnWarps * 32, sm, st>>>(p);
-    }
+    if (a.split) return a.groups == 1 ? launch_split<D, SP, 1>(p, a, rows, st) : launch_split<D, SP, 2>(p, a, rows, st);
+    static std::atomic<int> most[kMaxDev];
+    const int sm = kAttnWarps * (kTileGroups<D> * 3 * (D / 32) * 256 + 128 + Ring<D>::kBytes);
+    if (!allow_smem(k_attn_tiles<D, SP>, most, sm)) return ccuda("kv8_attention: shared memory");
+    k_attn_tiles<D, SP><<<dim3((unsigned) ((p.tiles + kAttnWarps - 1) / kAttnWarps), p.c.H, p.n_req), kAttnWarps * 32, sm, st>>>(p);
     return ccuda("kv8_attention");
 }
 
@@ -1151,9 +1231,8 @@ int tsb_block_tables(const int32_t* lens, const int32_t* n_new, const uint8_t* d
     const TabParams p{lens, n_new, done, n_req, table, table_stride, table_width, free_list, free_cap, n_free, block_size,
                       lens_out, cu_new, slots, cap_tokens, n_free_out};
     const int sm = 3 * (n_req + 1) * 4;
-    if (sm > 47 * 1024 &&
-        cudaFuncSetAttribute(k_block_tables, cudaFuncAttributeMaxDynamicSharedMemorySize, sm) != cudaSuccess)
-        return ccuda("block_tables: shared memory");
+    static std::atomic<int> most[kMaxDev];
+    if (!allow_smem(k_block_tables, most, sm)) return ccuda("block_tables: shared memory");
     const int64_t work = std::max<int64_t>(cap_tokens, n_req);
     const int ctas = (int) std::min<int64_t>(std::max<int64_t>((work + kTabThreads - 1) / kTabThreads, 1), std::max(sm_count(), 1));
     k_block_tables<<<ctas, kTabThreads, sm, cst(stream)>>>(p);
