@@ -12,6 +12,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtsb_moe.so")
+EXT = os.path.join(HERE, "_serving.so")          # the CPython module over the library (tinystrata_b200/serving.py)
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 SOURCES = ["tsb_moe.cu", "tsb_decode.cu", "tsb_decode_act.cu", "tsb_ep.cu", "tsb_staged.cu", "tsb_cache.cu",
            "tsb_delta.cu", "tsb_gguf.cpp"]
@@ -59,7 +60,32 @@ def build(verbose: bool = False, force: bool = False) -> str:
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
+    build_ext(verbose, force)
     return LIB
+
+
+def build_ext(verbose: bool = False, force: bool = False) -> str:
+    """The native Python module of the serving-step operators: C++ against torch's headers and the library beside it."""
+    import sysconfig
+
+    src = os.path.join(CSRC, "tsb_pyserving.cpp")
+    if not (force or _stale(EXT, [src, os.path.join(HERE, "..", "include", "tsb_moe.h")])):
+        return EXT
+    import torch
+    root = os.path.dirname(torch.__file__)
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], os.path.join(os.path.dirname(NVCC), "..", "include")]
+    libs = os.path.join(root, "lib")
+    cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *[f"-I{i}" for i in inc], src, "-o", EXT,
+           f"-L{HERE}", "-l:libtsb_moe.so", f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
+           "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed on tsb_pyserving.cpp:\n{r.stderr}")
+    return EXT
 
 
 if __name__ == "__main__":
