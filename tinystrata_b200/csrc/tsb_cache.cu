@@ -102,16 +102,18 @@ struct TabReq {
     int len, add, gives, has, takes;
     bool fits, done;
 };
+// Block counts in 32 bits: two lengths sum to less than 2^32.
+__device__ __forceinline__ unsigned blocks_of(unsigned n, unsigned bs) { return n ? (n - 1) / bs + 1 : 0; }
 __device__ __forceinline__ TabReq tab_req(const TabParams& p, int r) {
     TabReq q;
     q.len = max(p.lens[r], 0);
     q.add = max(p.n_new[r], 0);
     q.done = p.done && p.done[r] != 0;
-    q.has = (int) (((int64_t) q.len + p.block_size - 1) / p.block_size);
-    const int64_t after = ((int64_t) q.len + q.add + p.block_size - 1) / p.block_size;
-    q.fits = !q.done && after <= p.width;
+    q.has = (int) blocks_of(q.len, p.block_size);
+    const unsigned after = blocks_of((unsigned) q.len + (unsigned) q.add, p.block_size);
+    q.fits = !q.done && after <= (unsigned) p.width;
     q.gives = q.done ? min(q.has, p.width) : 0;
-    q.takes = q.fits ? (int) (after - q.has) : 0;
+    q.takes = q.fits ? (int) after - q.has : 0;
     return q;
 }
 
@@ -142,9 +144,11 @@ __global__ void __launch_bounds__(kTabThreads) k_block_tables(const TabParams p)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (R + kTabThreads - 1) / kTabThreads;
     const int r0 = min(tid * per, R), r1 = min(r0 + per, R);
+    const int held = min(max(*p.n_free, 0), p.cap_free);
     int s[3] = {0, 0, 0};
     for (int r = r0; r < r1; ++r) {
         const TabReq q = tab_req(p, r);
+        cu[r] = q.add, take[r] = q.takes, give[r] = q.gives;      // this thread's own, sums below
         s[0] += q.add, s[1] += q.takes, s[2] += q.gives;
     }
     int x[3];
@@ -165,14 +169,13 @@ __global__ void __launch_bounds__(kTabThreads) k_block_tables(const TabParams p)
         for (int w = 0; w < warp; ++w) x[i] += wsum[i][w];
     }
     for (int r = r0; r < r1; ++r) {
-        const TabReq q = tab_req(p, r);
+        const int add = cu[r], takes = take[r], gives = give[r];
         cu[r] = x[0], take[r] = x[1], give[r] = x[2];
-        x[0] += q.add, x[1] += q.takes, x[2] += q.gives;
+        x[0] += add, x[1] += takes, x[2] += gives;
     }
     if (tid == kTabThreads - 1) cu[R] = x[0], take[R] = x[1], give[R] = x[2];
     __syncthreads();
 
-    const int held = min(max(*p.n_free, 0), p.cap_free);
     const int given = min(give[R], p.cap_free - held);
     const int have = held + given;
     const int granted = take[last_le(take, R, have)];     // requests are served in order while their blocks last
@@ -192,7 +195,19 @@ __global__ void __launch_bounds__(kTabThreads) k_block_tables(const TabParams p)
         p.cu_new[R] = cu[R];
         *p.n_free_out = have - granted;
     }
-    for (int64_t i = g; i < given; i += step) p.free_list[held + i] = stack(held + (int) i);
+    for (int64_t i0 = g; i0 < given; i0 += 4 * step) {              // four table reads in flight
+        int b[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t i = i0 + u * step;
+            if (i >= given) break;
+            const int r = last_le(give, R, i);
+            b[u] = p.table[(int64_t) r * p.table_stride + (i - give[r])];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (i0 + u * step < given) p.free_list[held + i0 + u * step] = b[u];
+    }
     for (int64_t k = g; k < granted; k += step) {
         const int r = last_le(take, R, k);
         const TabReq q = tab_req(p, r);
@@ -204,11 +219,11 @@ __global__ void __launch_bounds__(kTabThreads) k_block_tables(const TabParams p)
             const int r = last_le(cu, R, t);
             const TabReq q = tab_req(p, r);
             if (q.fits && (q.takes == 0 || take[r + 1] <= have)) {
-                const int64_t pos = (int64_t) q.len + (t - cu[r]);
-                const int j = (int) (pos / p.block_size);
+                const unsigned pos = (unsigned) q.len + (unsigned) (t - cu[r]);
+                const int j = (int) (pos / (unsigned) p.block_size);
                 const int b = j < q.has ? p.table[(int64_t) r * p.table_stride + j]
                                         : stack(have - 1 - (take[r] + (j - q.has)));
-                slot = b < 0 ? -1 : (int64_t) b * p.block_size + pos % p.block_size;
+                slot = b < 0 ? -1 : (int64_t) b * p.block_size + (pos - (unsigned) j * (unsigned) p.block_size);
             }
         }
         p.slots[t] = slot;
@@ -219,7 +234,7 @@ __global__ void __launch_bounds__(kTabThreads) k_block_tables(const TabParams p)
 struct Cache {
     int8_t *k, *v;
     float *ks, *vs;
-    int n_blocks, bs, H, D;
+    int n_blocks, bs, H, D, shift;   // block_size = 1 << shift
 };
 
 struct AppendParams {
@@ -229,7 +244,6 @@ struct AppendParams {
     int64_t k_tok, k_head, v_tok, v_head;
     const int64_t* slots;
     int64_t n_tok;
-    int per_cta;      // tokens whose runs a CTA starts
     bool wide;
 };
 
@@ -244,115 +258,236 @@ __device__ __forceinline__ int cache_code(float x, float scale) {
     return scale > 0.0f ? (int) fminf(fmaxf(rintf(x / scale), -kCodeMax), kCodeMax) : 0;
 }
 
-// CTA (chunk of per_cta tokens, head).  A run is the tokens of one call that follow one another within one cache block;
-// its first token is the leader, and one warp takes a run's keys or values: the largest magnitude over the run, the
-// block's new scale max(old, largest / 127) (old: none when the run starts the block), the block's earlier codes
-// brought to it when it grew, and the run's codes.  One warp owns the (block, head), so no value is written twice and
-// nothing is atomic.  Divisions are IEEE: the same codes on any device.  Bound by the rows' bytes: the second pass over
-// a run reads it from L1.
-__global__ void __launch_bounds__(256) k_kv8_append(const AppendParams p) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int h = blockIdx.y;
-    const int bs = p.c.bs, D = p.c.D, DV = D / 8;
-    const int64_t t0 = (int64_t) blockIdx.x * p.per_cta, cap = (int64_t) p.c.n_blocks * bs;
-    const int64_t mine = t0 + lane;
-    bool leads = false;
-    if (lane < p.per_cta && mine < p.n_tok) {
-        const int64_t s = p.slots[mine];
-        if (s >= 0 && s < cap) leads = mine == 0 || s % bs == 0 || p.slots[mine - 1] != s - 1;
+// The largest magnitude bits of values that are stored as they are, for spotting the others (NaN, infinities) at once.
+constexpr uint32_t kPlainBits = 0x7f7f0000u;   // the largest finite bf16
+__device__ __forceinline__ uint32_t peak_bits(const float (&x)[8], uint32_t m) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+    return m;
+}
+__device__ __forceinline__ float peak_value(float (&x)[8]) {          // and the values as they are stored
+    uint32_t m = peak_bits(x, 0);
+    if (m > kPlainBits) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = cache_value(x[j]);
+        m = peak_bits(x, 0);
     }
-    unsigned todo = __ballot_sync(0xffffffffu, leads);
-    for (int job = 0; todo; ++job) {
-        const int at = __ffs(todo) - 1;
-        if (job & 1) todo &= todo - 1;
-        if ((job & 7) != warp) continue;
-        const bool is_v = job & 1;
-        const int64_t t = t0 + at, s = p.slots[t], blk = s / bs;
-        const int off = (int) (s - blk * bs);
-        int n = 0;                                       // tokens of the run
-        for (int base = 0; base < bs - off; base += 32) {
-            const int i = base + lane;
-            const bool in = i < bs - off && t + i < p.n_tok && p.slots[t + i] == s + i;
-            const unsigned b = __ballot_sync(0xffffffffu, in);
-            n += b == 0xffffffffu ? 32 : __ffs(~b) - 1;
-            if (b != 0xffffffffu) break;
+    return __uint_as_float(m);
+}
+// Eight codes of plain values: rint(x / scale) as the division gives it.  The product with the reciprocal is within
+// 3 * 2^-24 * 127 of the quotient, so unless it lies that near to half way between two whole numbers both round alike;
+// adding 1.5 * 2^23 rounds to even and leaves the code in the low byte.  (The division itself bound the kernel: 82 us
+// for 16,024 tokens of 8 heads.)
+__device__ __forceinline__ uint2 encode8(const float (&x)[8], float scale, float inv) {
+    uint32_t u[2];
+    float far = scale > 1e-30f ? 0.0f : 1.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        uint32_t t[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float q = x[4 * i + j] * inv, r = q + 12582912.0f;
+            t[j] = __float_as_uint(r);
+            far = fmaxf(far, fabsf(q - (r - 12582912.0f)));
         }
-        const void* src = is_v ? p.v : p.k;
-        const int64_t row = is_v ? p.v_tok : p.k_tok, col = (is_v ? p.v_head : p.k_head) * h;
-        int8_t* codes = (is_v ? p.c.v : p.c.k) + (blk * p.c.H + h) * (int64_t) bs * D;
-        float* sp = (is_v ? p.c.vs : p.c.ks) + blk * p.c.H + h;
-        float peak = 0.0f;
-        for (int e = lane; e < n * DV; e += 32) {
-            float x[8];
-            load8(x, src, (t + e / DV) * row + col + (e % DV) * 8, p.type, p.wide);
+        u[i] = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+    }
+    if (far > 0.4998f) {
+        u[0] = u[1] = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) peak = fmaxf(peak, fabsf(cache_value(x[j])));
+        for (int j = 0; j < 8; ++j) u[j >> 2] |= (uint32_t) (uint8_t) cache_code(x[j], scale) << (8 * (j & 3));
+    }
+    return make_uint2(u[0], u[1]);
+}
+
+// 16 codes under a scale that grew: ratio = old / new.
+__device__ __forceinline__ uint4 rescale_codes(uint4 w, float ratio) {
+    uint32_t* u = (uint32_t*) &w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t r = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r |= (uint32_t) (uint8_t) (int8_t) rintf((float) (int8_t) (u[i] >> (8 * j)) * ratio) << (8 * j);
+        u[i] = r;
+    }
+    return w;
+}
+
+// Warp (keys or values, head, token), for decode steps, where nearly every token is a run of its own.  A run is the tokens of one call that follow one another within one
+// cache block; its first token is the leader, and its warp takes the run: the largest magnitude over
+// it, the block's new scale max(old, largest / 127) (old: none when the run starts the block), the block's earlier codes
+// brought to it when it grew, and the run's codes.  One warp owns the (block, head), so no value is written twice and
+// nothing is atomic.  Divisions are IEEE: the same codes on any device.  Bound by the chain of loads: slots, rows, scale.
+__global__ void __launch_bounds__(128) k_kv8_append(const AppendParams p) {
+    const int lane = threadIdx.x & 31;
+    const int bs = p.c.bs, D = p.c.D, DV = D / 8, dvs = D == 64 ? 3 : D == 128 ? 4 : 5;
+    const int64_t cap = (int64_t) p.c.n_blocks << p.c.shift;
+    const unsigned part = blockIdx.x / p.c.H;
+    const int h = (int) (blockIdx.x - part * p.c.H);
+    const bool is_v = part & 1;
+    const int64_t t = (int64_t) (part >> 1) * 4 + (threadIdx.x >> 5);
+    if (t >= p.n_tok) return;
+    const void* src = is_v ? p.v : p.k;
+    const int64_t row = is_v ? p.v_tok : p.k_tok, col = (is_v ? p.v_head : p.k_head) * h;
+    const int64_t s = p.slots[t], before = t ? p.slots[t - 1] : -2;
+    if (s < 0 || s >= cap || ((s & (bs - 1)) && before == s - 1)) return;
+    const int64_t blk = s >> p.c.shift;
+    const int off = (int) (s & (bs - 1));
+    int n = 0;                                       // tokens of the run
+    for (int b0 = 0; b0 < bs - off; b0 += 32) {
+        const int i = b0 + lane;
+        const bool in = i < bs - off && t + i < p.n_tok && p.slots[t + i] == s + i;
+        const unsigned b = __ballot_sync(0xffffffffu, in);
+        n += b == 0xffffffffu ? 32 : __ffs(~b) - 1;
+        if (b != 0xffffffffu) break;
+    }
+    int8_t* codes = (is_v ? p.c.v : p.c.k) + ((blk * p.c.H + h) << p.c.shift) * D;
+    float* sp = (is_v ? p.c.vs : p.c.ks) + blk * p.c.H + h;
+    const float was = off > 0 ? *sp : 0.0f;
+    float peak = 0.0f;
+#pragma unroll 4
+    for (int e = lane; e < n * DV; e += 32) {
+        float x[8];
+        load8(x, src, (t + (e >> dvs)) * row + col + (e & (DV - 1)) * 8, p.type, p.wide);
+        peak = fmaxf(peak, peak_value(x));
+    }
+    peak = warp_max(peak);
+    const float now = fmaxf(was, peak / kCodeMax), inv = 1.0f / now;
+    __syncwarp();
+    if (lane == 0) *sp = now;
+    if (off > 0 && now != was) {
+        const float ratio = was / now;
+        for (int e = lane; e < off * D / 16; e += 32) ((uint4*) codes)[e] = rescale_codes(((const uint4*) codes)[e], ratio);
+    }
+#pragma unroll 4
+    for (int e = lane; e < n * DV; e += 32) {
+        float x[8];
+        load8(x, src, (t + (e >> dvs)) * row + col + (e & (DV - 1)) * 8, p.type, p.wide);
+        peak_value(x);
+        *(uint2*) (codes + (int64_t) off * D + (int64_t) e * 8) = encode8(x, now, inv);
+    }
+}
+
+// The same for prompts: CTA (chunk of block_size tokens, head, keys or values), the run's values in registers between the
+// two passes (up to 64 a thread; a warp's two passes over 16 KB went to memory twice: 82 us for 16,024 tokens of 8 heads).
+__global__ void __launch_bounds__(128) k_kv8_append_runs(const AppendParams p) {
+    __shared__ float peaks[4];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int bs = p.c.bs, D = p.c.D, DV = D / 8, dvs = D == 64 ? 3 : D == 128 ? 4 : 5;
+    const int64_t cap = (int64_t) p.c.n_blocks << p.c.shift;
+    // heads vary fastest: neighbouring CTAs read a token's whole row
+    const unsigned part = blockIdx.x / p.c.H;
+    const int h = (int) (blockIdx.x - part * p.c.H);
+    const bool is_v = part & 1;
+    const int64_t start = (int64_t) (part >> 1) * bs, end_t = min(start + bs, p.n_tok);
+    const void* src = is_v ? p.v : p.k;
+    const int64_t row = is_v ? p.v_tok : p.k_tok, col = (is_v ? p.v_head : p.k_head) * h;
+    for (int64_t base_t = start; base_t < end_t; base_t += 32) {          // every warp finds the leaders for itself
+        const int64_t mine = base_t + lane;
+        bool leads = false;
+        if (mine < end_t) {
+            const int64_t s = p.slots[mine], before = mine ? p.slots[mine - 1] : -2;
+            leads = s >= 0 && s < cap && ((s & (bs - 1)) == 0 || before != s - 1);
         }
-        peak = warp_max(peak);
-        const float was = off > 0 ? *sp : 0.0f;
-        const float now = fmaxf(was, peak / kCodeMax);
-        __syncwarp();
-        if (lane == 0) *sp = now;
-        if (off > 0 && now != was) {
-            const float ratio = was / now;
-            for (int e = lane; e < off * D / 16; e += 32) {
-                uint4 w = ((const uint4*) codes)[e];
-                uint32_t* u = (uint32_t*) &w;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t r = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        r |= (uint32_t) (uint8_t) (int8_t) rintf((float) (int8_t) (u[i] >> (8 * j)) * ratio) << (8 * j);
-                    u[i] = r;
-                }
-                ((uint4*) codes)[e] = w;
+        for (unsigned todo = __ballot_sync(0xffffffffu, leads); todo; todo &= todo - 1) {
+            const int64_t t = base_t + __ffs(todo) - 1, s = p.slots[t], blk = s >> p.c.shift;
+            const int off = (int) (s & (bs - 1));
+            int n = 0;
+            for (int b0 = 0; b0 < bs - off; b0 += 32) {
+                const int i = b0 + lane;
+                const bool in = i < bs - off && t + i < p.n_tok && p.slots[t + i] == s + i;
+                const unsigned b = __ballot_sync(0xffffffffu, in);
+                n += b == 0xffffffffu ? 32 : __ffs(~b) - 1;
+                if (b != 0xffffffffu) break;
             }
-        }
-        for (int e = lane; e < n * DV; e += 32) {
-            float x[8];
-            load8(x, src, (t + e / DV) * row + col + (e % DV) * 8, p.type, p.wide);
-            uint32_t u[2] = {0, 0};
+            int8_t* codes = (is_v ? p.c.v : p.c.k) + ((blk * p.c.H + h) << p.c.shift) * D;
+            float* sp = (is_v ? p.c.vs : p.c.ks) + blk * p.c.H + h;
+            const float was = off > 0 ? *sp : 0.0f;
+            constexpr int HOLD = 8;
+            float x[HOLD][8], peak = 0.0f;
+            auto at = [&](int e) { return (t + (e >> dvs)) * row + col + (e & (DV - 1)) * 8; };
 #pragma unroll
-            for (int j = 0; j < 8; ++j) u[j >> 2] |= (uint32_t) (uint8_t) cache_code(cache_value(x[j]), now) << (8 * (j & 3));
-            *(uint2*) (codes + (int64_t) off * D + (int64_t) e * 8) = make_uint2(u[0], u[1]);
+            for (int i = 0; i < HOLD; ++i) {
+                const int e = i * 128 + tid;
+                if (e < n * DV) load8(x[i], src, at(e), p.type, p.wide);
+            }
+#pragma unroll
+            for (int i = 0; i < HOLD; ++i) {
+                if (i * 128 + tid >= n * DV) break;
+                peak = fmaxf(peak, peak_value(x[i]));
+            }
+            for (int e = HOLD * 128 + tid; e < n * DV; e += 128) {         // longer runs: the rest is read twice
+                float y[8];
+                load8(y, src, at(e), p.type, p.wide);
+                peak = fmaxf(peak, peak_value(y));
+            }
+            peak = warp_max(peak);
+            if (lane == 0) peaks[warp] = peak;
+            __syncthreads();                                               // also: every thread has read the old scale
+            peak = fmaxf(fmaxf(peaks[0], peaks[1]), fmaxf(peaks[2], peaks[3]));
+            const float now = fmaxf(was, peak / kCodeMax), inv = 1.0f / now;
+            if (tid == 0) *sp = now;
+            if (off > 0 && now != was) {
+                const float ratio = was / now;
+                for (int e = tid; e < off * D / 16; e += 128) ((uint4*) codes)[e] = rescale_codes(((const uint4*) codes)[e], ratio);
+            }
+            auto put = [&](int e, const float (&y)[8]) {
+                *(uint2*) (codes + (int64_t) off * D + (int64_t) e * 8) = encode8(y, now, inv);
+            };
+#pragma unroll
+            for (int i = 0; i < HOLD; ++i) {
+                const int e = i * 128 + tid;
+                if (e < n * DV) put(e, x[i]);
+            }
+            for (int e = HOLD * 128 + tid; e < n * DV; e += 128) {
+                float y[8];
+                load8(y, src, at(e), p.type, p.wide);
+                peak_value(y);
+                put(e, y);
+            }
+            __syncthreads();                                               // peaks are read
         }
     }
 }
 
-// One thread per 16 values of a (token, head): key and value.  A slot outside the cache reads as zeros.
+// CTA (share of the tokens, head, keys or values): four codes a thread and step, so that a warp's stores of 16 (8) bytes a
+// lane are consecutive, eight steps in flight.  A slot outside the cache reads as zeros.
+constexpr int kReadSteps = 8;
 __global__ void __launch_bounds__(256) k_kv8_read(const Cache c, const int64_t* __restrict__ slots, int64_t n_tok,
                                                   void* k, void* v, int type) {
-    const int per = c.D / 16;
-    const int64_t e = (int64_t) blockIdx.x * 256 + threadIdx.x;
-    if (e >= n_tok * c.H * per) return;
-    const int64_t th = e / per, t = th / c.H;
-    const int h = (int) (th - t * c.H), part = (int) (e - th * per);
-    const int64_t s = slots[t];
-    const bool ok = s >= 0 && s < (int64_t) c.n_blocks * c.bs;
-    const int64_t blk = ok ? s / c.bs : 0, bh = blk * c.H + h;
+    const int per = c.D / 4, ps = c.D == 64 ? 4 : c.D == 128 ? 5 : 6;
+    const unsigned share = blockIdx.x / c.H;             // heads vary fastest, as the outputs' rows do
+    const int h = (int) (blockIdx.x - share * c.H);
+    const bool is_v = share & 1;
+    const int8_t* codes = is_v ? c.v : c.k;
+    const float* scales = is_v ? c.vs : c.ks;
+    void* out = is_v ? v : k;
+    const int64_t cap = (int64_t) c.n_blocks << c.shift;
+    const int64_t e0 = (int64_t) (share >> 1) * 256 * kReadSteps + threadIdx.x;
+    uint32_t w[kReadSteps];
+    float sc[kReadSteps];
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-        const int8_t* codes = (w ? c.v : c.k) + (bh * c.bs + (ok ? s - blk * c.bs : 0)) * c.D + part * 16;
-        const uint4 q = ok ? *(const uint4*) codes : make_uint4(0, 0, 0, 0);
-        const float sc = ok ? (w ? c.vs : c.ks)[bh] : 0.0f;
-        const uint32_t u[4] = {q.x, q.y, q.z, q.w};
-        float f[16];
+    for (int i = 0; i < kReadSteps; ++i) {
+        const int64_t e = e0 + i * 256, t = e >> ps;
+        w[i] = 0, sc[i] = 0.0f;
+        if (t >= n_tok) continue;
+        const int64_t s = slots[t];
+        if (s < 0 || s >= cap) continue;
+        const int64_t bh = (s >> c.shift) * c.H + h;
+        w[i] = *(const uint32_t*) (codes + ((bh << c.shift) + (s & (c.bs - 1))) * c.D + (e & (per - 1)) * 4);
+        sc[i] = scales[bh];
+    }
 #pragma unroll
-        for (int j = 0; j < 16; ++j) f[j] = (float) (int8_t) (u[j >> 2] >> (8 * (j & 3))) * sc;
-        void* out = w ? v : k;
-        if (type == E_F32) {
+    for (int i = 0; i < kReadSteps; ++i) {
+        const int64_t e = e0 + i * 256, t = e >> ps;
+        if (t >= n_tok) break;
+        const int64_t at = (t * c.H + h) * c.D + (e & (per - 1)) * 4;
+        float f[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                ((float4*) out)[e * 4 + j] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
-        } else {
-            uint32_t r[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                r[j] = type == E_F16 ? pack_f16(f[2 * j], f[2 * j + 1]) : pack_bf16(f[2 * j], f[2 * j + 1]);
-            ((uint4*) out)[e * 2] = make_uint4(r[0], r[1], r[2], r[3]);
-            ((uint4*) out)[e * 2 + 1] = make_uint4(r[4], r[5], r[6], r[7]);
-        }
+        for (int j = 0; j < 4; ++j) f[j] = (float) (int8_t) (w[i] >> (8 * j)) * sc[i];
+        if (type == E_F32) *(float4*) ((float*) out + at) = make_float4(f[0], f[1], f[2], f[3]);
+        else if (type == E_F16) *(uint2*) ((uint16_t*) out + at) = make_uint2(pack_f16(f[0], f[1]), pack_f16(f[2], f[3]));
+        else *(uint2*) ((uint16_t*) out + at) = make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]));
     }
 }
 
@@ -1142,7 +1277,8 @@ int check_cache(const tsb_kv8* c, const char* what) {
     return TSB_OK;
 }
 Cache cache_of(const tsb_kv8* c) {
-    return Cache{c->k, c->v, c->k_scale, c->v_scale, c->n_blocks, c->block_size, c->n_kv_heads, c->head_dim};
+    return Cache{c->k, c->v, c->k_scale, c->v_scale, c->n_blocks, c->block_size, c->n_kv_heads, c->head_dim,
+                 c->block_size == 16 ? 4 : c->block_size == 32 ? 5 : 6};
 }
 bool elem_ok(int t) { return t == E_F32 || t == E_F16 || t == E_BF16; }
 
@@ -1233,8 +1369,9 @@ int tsb_block_tables(const int32_t* lens, const int32_t* n_new, const uint8_t* d
     const int sm = 3 * (n_req + 1) * 4;
     static std::atomic<int> most[kMaxDev];
     if (!allow_smem(k_block_tables, most, sm)) return ccuda("block_tables: shared memory");
-    const int64_t work = std::max<int64_t>(cap_tokens, n_req);
-    const int ctas = (int) std::min<int64_t>(std::max<int64_t>((work + kTabThreads - 1) / kTabThreads, 1), std::max(sm_count(), 1));
+    // a thread a token, and for blocks that may be given back
+    const int64_t work = std::max<int64_t>({cap_tokens, n_req, (int64_t) n_req * table_width / 16});
+    const int ctas = (int) std::min<int64_t>(std::max<int64_t>((work + kTabThreads - 1) / kTabThreads, 1), std::max(2 * sm_count(), 1));
     k_block_tables<<<ctas, kTabThreads, sm, cst(stream)>>>(p);
     return ccuda("block_tables");
 }
@@ -1249,13 +1386,16 @@ int tsb_kv8_append(const tsb_kv8* cache, const void* k, const void* v, int elem_
     const int es = elem_bytes(elem_type);
     if ((uintptr_t) k % es || (uintptr_t) v % es) return cfail(TSB_ERR_ALIGN, "kv8_append: element alignment");
     if (cache->n_kv_heads > 65535) return cfail(TSB_ERR_UNSUPPORTED, "kv8_append: at most 65535 heads");
-    AppendParams p{cache_of(cache), k, v, elem_type, k_tok, k_head, v_tok, v_head, slots, n_tok, 0, false};
+    AppendParams p{cache_of(cache), k, v, elem_type, k_tok, k_head, v_tok, v_head, slots, n_tok, false};
     p.wide = !((uintptr_t) k % 16 || (uintptr_t) v % 16 || (k_tok * es) % 16 || (k_head * es) % 16 || (v_tok * es) % 16 ||
                (v_head * es) % 16);
-    p.per_cta = n_tok <= 1024 ? 4 : 32;
-    const int64_t chunks = (n_tok + p.per_cta - 1) / p.per_cta;
-    if (chunks > 0x7fffffffll) return cfail(TSB_ERR_UNSUPPORTED, "kv8_append: too many tokens");
-    k_kv8_append<<<dim3((unsigned) chunks, cache->n_kv_heads), 256, 0, cst(stream)>>>(p);
+    // few tokens are decode steps, a run each: a warp a token; many are prompts: a CTA a block's worth
+    const bool few = n_tok <= 1024;
+    const int64_t ctas = few ? (n_tok + 3) / 4 : (n_tok + cache->block_size - 1) / cache->block_size;
+    if (ctas > 0x7fffffffll / 2 / cache->n_kv_heads) return cfail(TSB_ERR_UNSUPPORTED, "kv8_append: too many tokens");
+    const unsigned grid = (unsigned) (ctas * 2 * cache->n_kv_heads);
+    if (few) k_kv8_append<<<grid, 128, 0, cst(stream)>>>(p);
+    else k_kv8_append_runs<<<grid, 128, 0, cst(stream)>>>(p);
     return ccuda("kv8_append");
 }
 
@@ -1266,9 +1406,9 @@ int tsb_kv8_read(const tsb_kv8* cache, const int64_t* slots, int64_t n_tok, void
     if (n_tok == 0) return TSB_OK;
     if (!k || !v || !slots) return cfail(TSB_ERR_ARG, "kv8_read: null pointer");
     if ((uintptr_t) k % 16 || (uintptr_t) v % 16) return cfail(TSB_ERR_ALIGN, "kv8_read: 16-byte aligned outputs");
-    const int64_t n = n_tok * cache->n_kv_heads * (cache->head_dim / 16), ctas = (n + 255) / 256;
-    if (ctas > 0x7fffffffll) return cfail(TSB_ERR_UNSUPPORTED, "kv8_read: too many tokens");
-    k_kv8_read<<<(unsigned) ctas, 256, 0, cst(stream)>>>(cache_of(cache), slots, n_tok, k, v, elem_type);
+    const int64_t ctas = (n_tok * (cache->head_dim / 4) + 256 * kReadSteps - 1) / (256 * kReadSteps);
+    if (ctas > 0x7fffffffll / 2 / cache->n_kv_heads) return cfail(TSB_ERR_UNSUPPORTED, "kv8_read: too many tokens");
+    k_kv8_read<<<(unsigned) (ctas * 2 * cache->n_kv_heads), 256, 0, cst(stream)>>>(cache_of(cache), slots, n_tok, k, v, elem_type);
     return ccuda("kv8_read");
 }
 

@@ -91,12 +91,17 @@ __device__ __forceinline__ int state_of(const DeltaParams& p, int b) {
 }
 
 // ------------------------------------------------------------------------------------------------ recurrence
+__device__ __forceinline__ float4 ld_state(const float* p) {     // volatile: issued where it stands
+    float4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+    return v;
+}
 // CTA (32 value columns, value head, sequence): the state's slice in registers, thread (row group of 32, 4 columns):
 // dim_k / 32 rows of four columns.  One reduction over dim_k a token: S^T k and S^T q of the decayed state together,
 // o = scale (S^T q + (q . k) u), so the second product needs no second pass.  Single tokens are bound by the state's
 // bytes, read and written once.
 template <int DK>
-__global__ void __launch_bounds__(256) k_delta_step(const DeltaParams p) {
+__global__ void __launch_bounds__(256, 4) k_delta_step(const DeltaParams p) {
     constexpr int RPT = DK / 32;
     __shared__ float qk[2][DK];
     __shared__ float red[8][2][32];
@@ -104,8 +109,6 @@ __global__ void __launch_bounds__(256) k_delta_step(const DeltaParams p) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int c4 = (tid & 7) * 4, rg = tid >> 3;
     const int col = blockIdx.x * 32 + c4, h = blockIdx.y, b = blockIdx.z;
-    const Seq s = seq_of(p, b);
-    if (s.n == 0 && p.s_in == p.s_out) return;
     const int st = state_of(p, b);
     const int hk = h / (p.hv / p.hk);
     const int64_t base = ((int64_t) max(st, 0) * p.hv + h) * DK * p.dv + col;
@@ -113,7 +116,9 @@ __global__ void __launch_bounds__(256) k_delta_step(const DeltaParams p) {
     float4 S[RPT];
 #pragma unroll
     for (int i = 0; i < RPT; ++i)
-        S[i] = st >= 0 && in ? __ldcs((const float4*) (p.s_in + base + (int64_t) (i * 32 + rg) * p.dv)) : make_float4(0, 0, 0, 0);
+        S[i] = st >= 0 && in ? ld_state(p.s_in + base + (int64_t) (i * 32 + rg) * p.dv) : make_float4(0, 0, 0, 0);
+    const Seq s = seq_of(p, b);      // after the state's loads are on their way: nothing before them waits for memory
+    if (s.n == 0 && p.s_in == p.s_out) return;
     for (int t = 0; t < s.n; ++t) {
         const int64_t tok = s.tok + t;
         float dkk = 0.0f, dqq = 0.0f, dqk = 0.0f;
