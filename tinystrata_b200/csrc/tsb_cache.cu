@@ -494,8 +494,7 @@ __global__ void __launch_bounds__(256) k_kv8_read(const Cache c, const int64_t* 
 // ------------------------------------------------------------------------------------------------ attention
 constexpr int kAttnWarps = 4;
 constexpr int kStep = 16;            // tokens of a step: one matrix-product depth, always within one cache block
-constexpr int kSplitRows = 64;       // rows a key / value head has (queries x heads of its group) up to which the
-                                     // steps of a request are split over CTAs
+constexpr int kSplitRows = 64, kSplitMost = 1024, kPromptCtas = 24;   // see attn_plan
 constexpr int kMaxReq = 4096;
 
 struct AttnParams {
@@ -515,6 +514,7 @@ struct AttnParams {
     float* part;                     // [2 * CTAs][tile rows][D], then their maxima and sums [2 * CTAs][2][tile rows]
     int n_cta;
     bool wide_out;                   // 16-byte aligned output rows
+    unsigned* err;
 };
 
 struct Req {
@@ -1263,6 +1263,13 @@ __global__ void __launch_bounds__(kAttnWarps * 32) k_attn_tiles(const __grid_con
         }
 }
 
+}  // namespace
+}  // namespace tsb
+#include "tsb_cache_prompt.cuh"
+namespace tsb {
+unsigned* device_error_word();          // tsb_moe.cu: the current device's error word
+namespace {
+
 // ------------------------------------------------------------------------------------------------ host
 int check_cache(const tsb_kv8* c, const char* what) {
     if (!c || c->struct_size != sizeof(tsb_kv8)) return cfail(TSB_ERR_ARG, "%s: cache struct_size", what);
@@ -1284,7 +1291,7 @@ bool elem_ok(int t) { return t == E_F32 || t == E_F16 || t == E_BF16; }
 
 struct AttnPlan {
     int G, tiles, n_cta, groups;
-    bool split;
+    bool split, prompt;
     uint64_t ws;
 };
 int attn_plan(const tsb_kv8* c, const tsb_kv8_attn* d, AttnPlan& a) {
@@ -1301,8 +1308,13 @@ int attn_plan(const tsb_kv8* c, const tsb_kv8_attn* d, AttnPlan& a) {
     a.G = d->q_heads / c->n_kv_heads;
     const int64_t rows = (int64_t) d->max_q * a.G;
     if (rows > (1 << 28)) return cfail(TSB_ERR_UNSUPPORTED, "kv8_attention: too many query rows");
-    a.split = rows <= kSplitRows;
-    a.groups = !a.split ? (c->head_dim == 256 ? kTileGroups<256> : kTileGroups<128>) : rows <= 8 ? 1 : 2;
+    // Rows a key / value head has (queries x heads of its group).  Up to 64 the steps of a request are split over CTAs; above,
+    // tiles of rows walk all of their keys, 16-bit queries in tiles of 128 on tcgen05.  A few hundred rows whose tiles would
+    // leave most SMs idle are split too.
+    const int64_t prompt_ctas = (rows + 127) / 128 * c->n_kv_heads * d->n_req;
+    a.split = rows <= kSplitRows || (rows <= kSplitMost && prompt_ctas < kPromptCtas);
+    a.prompt = !a.split && d->elem_type != E_F32;
+    a.groups = a.prompt ? 16 : !a.split ? (c->head_dim == 256 ? kTileGroups<256> : kTileGroups<128>) : rows <= 8 ? 1 : 2;
     a.tiles = (int) ((rows + 8 * a.groups - 1) / (8 * a.groups));
     const int sms = sm_count();
     if (!sms) return cfail(TSB_ERR_CUDA, "kv8_attention: no CUDA device");
@@ -1337,6 +1349,12 @@ int launch_split(const AttnParams& p, const AttnPlan& a, int rows, cudaStream_t 
 template <int D, int SP>
 int launch_attn(const AttnParams& p, const AttnPlan& a, int rows, cudaStream_t st) {
     if (a.split) return a.groups == 1 ? launch_split<D, SP, 1>(p, a, rows, st) : launch_split<D, SP, 2>(p, a, rows, st);
+    if constexpr (SP == 1) {
+        static std::atomic<int> most[kMaxDev];
+        if (!allow_smem(k_attn_prompt<D>, most, Prompt<D>::kAsk)) return ccuda("kv8_attention: shared memory");
+        k_attn_prompt<D><<<dim3((unsigned) p.tiles, p.c.H, p.n_req), kPromptThreads, Prompt<D>::kAsk, st>>>(p);
+        return ccuda("kv8_attention");
+    }
     static std::atomic<int> most[kMaxDev];
     const int sm = kAttnWarps * (kTileGroups<D> * 3 * (D / 32) * 256 + 128 + Ring<D>::kBytes);
     if (!allow_smem(k_attn_tiles<D, SP>, most, sm)) return ccuda("kv8_attention: shared memory");
@@ -1345,6 +1363,12 @@ int launch_attn(const AttnParams& p, const AttnPlan& a, int rows, cudaStream_t s
 }
 
 }  // namespace
+
+// This file's copy of the bound of the waits (tsb_set_wait_limit_ns writes each).
+int cache_set_wait_limit(unsigned long long ns) {
+    return cudaMemcpyToSymbol(g_wait_ns, &ns, sizeof ns) == cudaSuccess ? TSB_OK : TSB_ERR_CUDA;
+}
+
 }  // namespace tsb
 
 using namespace tsb;
@@ -1439,7 +1463,7 @@ int tsb_kv8_attention(const tsb_kv8* cache, const tsb_kv8_attn* d, const void* q
     p.scale_log2 = d->scale * 1.4426950408889634f;
     p.q_tok = d->q_tok, p.q_head = d->q_head, p.o_tok = d->o_tok, p.o_head = d->o_head, p.n_tok = d->n_tok;
     p.table = table, p.table_stride = d->table_stride, p.width = d->table_width, p.lens = lens, p.cu = cu_q;
-    p.tiles = a.tiles, p.n_cta = a.n_cta;
+    p.tiles = a.tiles, p.n_cta = a.n_cta, p.err = device_error_word();
     p.pre = (int64_t*) workspace;
     p.part = (float*) ((uint8_t*) workspace + (((uint64_t) d->n_req + 1) * 8 + 255) / 256 * 256);
     p.wide_out = !((uintptr_t) out % 16 || (d->o_tok * es) % 16 || (d->o_head * es) % 16);

@@ -21,6 +21,7 @@ namespace tsb {
 int decode_set_wait_limit(unsigned long long ns);   // tsb_decode.cu: that translation unit's copy of the bound
 int decode_act_set_wait_limit(unsigned long long ns);   // tsb_decode_act.cu: its copy of the bound
 int delta_set_wait_limit(unsigned long long ns);        // tsb_delta.cu: its copy of the bound
+int cache_set_wait_limit(unsigned long long ns);        // tsb_cache.cu: its copy of the bound
 
 // ================================================================================================ host error state
 static thread_local char g_err[512] = "";
@@ -621,6 +622,7 @@ int tsb_set_wait_limit_ns(uint64_t ns) {
     if (decode_set_wait_limit(v) != TSB_OK) return cuda_status("set_wait_limit_ns (decode)");
     if (decode_act_set_wait_limit(v) != TSB_OK) return cuda_status("set_wait_limit_ns (decode_act)");
     if (delta_set_wait_limit(v) != TSB_OK) return cuda_status("set_wait_limit_ns (delta)");
+    if (cache_set_wait_limit(v) != TSB_OK) return cuda_status("set_wait_limit_ns (cache)");
     return TSB_OK;
 }
 

@@ -1,34 +1,13 @@
 // tsb_prefill.cuh - the prefill (many-token) expert path's building blocks: the dispatch of routed entries into
-// expert-contiguous rows (the reference's permutation, src/qwen35/q36_engine.cu:486-510), and the tcgen05 / TMEM
-// helpers the tensor-core grouped products (tsb_mmq.cuh) issue.
+// expert-contiguous rows (the reference's permutation, src/qwen35/q36_engine.cu:486-510).
 #pragma once
 
 #include "tsb_kernels.cuh"
+#include "tsb_tc.cuh"
 
 #include <cuda_fp16.h>
 
 namespace tsb {
-
-// ------------------------------------------------------------------------------------------------ PTX helpers
-// Shared-memory matrix descriptor of a K-major operand tile with the 128-byte swizzle: 8-row groups 1 KB apart.
-__device__ __forceinline__ uint64_t pf_sdesc(uint32_t addr) {
-    return (uint64_t) ((addr >> 4) & 0x3FFFu) | ((uint64_t) 1 << 16) | ((uint64_t) (1024 >> 4) << 32) |
-           ((uint64_t) 1 << 46) | ((uint64_t) 2 << 61);
-}
-// The mbarrier arrives once every tcgen05.mma this thread issued before it has completed.
-__device__ __forceinline__ void pf_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-// byte offset of the 16-byte chunk c (values 8c..8c+7) of row r inside a K-major 128-byte-swizzled tile
-__device__ __forceinline__ uint32_t sw128(int r, int c) {
-    return (uint32_t) ((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4));
-}
-
 
 // ------------------------------------------------------------------------------------------------ dispatch
 // bounds[e] = number of entries routed to experts < e (bounds[E] = the entries placed); one CTA.
