@@ -712,9 +712,9 @@ __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 
 // products, registers and exponentials.  x = q . k (int8 products, exact) times the block's key scale and the row's; the
 // online softmax's largest score m and sum l in fp32 (the lanes compare their scores with m; only when one is larger do
 // they meet); o += weights . codes times the block's value scale.
-// SP 1, 16-bit outputs: weights, times 2^15 and the value scale relative to the largest so far, enter the product as one
+// SP 1, bf16 outputs: weights, times 2^15 and the value scale relative to the largest so far, enter the product as one
 //   fp16 value (11 bits down to 2^-29 of the largest weight; 2^-40 of it below) and o accumulates in the tensor cores.
-// SP 2, fp32 outputs: weights as two fp16 values; a step's product starts from zero and is added in fp32 times the value
+// SP 2, fp32 and fp16 outputs: weights as two fp16 values; a step's product starts from zero and is added in fp32 times the value
 //   scale, since the tensor cores' sums truncate.
 template <int D, int SP>
 struct Walk {
@@ -1216,12 +1216,12 @@ __global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ AttnP
     }
 }
 
-// Many rows: one warp per tile of 32 rows (head_dim 256: 16), every step of the tile by the same warp, which turns a
+// Many rows of fp32 queries: one warp per tile of 32 rows (head_dim 256: 16), every step of the tile by the same warp, which turns a
 // step's codes into operands once for all of them; the four warps of a CTA take neighbouring tiles of a head, so they share
 // the codes through the caches.
 template <int D>
 constexpr int kTileGroups = D == 256 ? 2 : 4;
-template <int D, int SP>
+template <int D>
 __global__ void __launch_bounds__(kAttnWarps * 32) k_attn_tiles(const __grid_constant__ AttnParams p) {
     constexpr int NB = kTileGroups<D>, TR = 8 * NB;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -1235,7 +1235,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) k_attn_tiles(const __grid_con
     if (rt * TR >= q.n * p.G) return;
     int first, n;
     tile_steps<TR>(p, q, rt, first, n);
-    Walk<D, SP> walk(p, smem_u32(ring), r, h, first, n, 0, 1, lane);
+    Walk<D, 2> walk(p, smem_u32(ring), r, h, first, n, 0, 1, lane);
     stage_rows<D, NB>(p, q, h, rt, qf, rowf, 0, 1, lane);
     __syncwarp();
     Rows<D, NB> rows;
@@ -1346,19 +1346,23 @@ int launch_split(const AttnParams& p, const AttnPlan& a, int rows, cudaStream_t 
     cudaLaunchKernelEx(&cfg, k_attn_join<D, 8 * NB>, p);
     return ccuda("kv8_attention: join");
 }
+template <int D, bool LO>
+int launch_prompt(const AttnParams& p, cudaStream_t st) {
+    static std::atomic<int> most[kMaxDev];
+    if (!allow_smem(k_attn_prompt<D, LO>, most, Prompt<D, LO>::kAsk)) return ccuda("kv8_attention: shared memory");
+    k_attn_prompt<D, LO><<<dim3((unsigned) p.tiles, p.c.H, p.n_req), kPromptThreads, Prompt<D, LO>::kAsk, st>>>(p);
+    return ccuda("kv8_attention");
+}
 template <int D, int SP>
 int launch_attn(const AttnParams& p, const AttnPlan& a, int rows, cudaStream_t st) {
     if (a.split) return a.groups == 1 ? launch_split<D, SP, 1>(p, a, rows, st) : launch_split<D, SP, 2>(p, a, rows, st);
-    if constexpr (SP == 1) {
+    if (a.prompt) return launch_prompt<D, SP == 2>(p, st);
+    if constexpr (SP == 2) {                 // fp32 queries (a 16-bit prompt went to launch_prompt)
         static std::atomic<int> most[kMaxDev];
-        if (!allow_smem(k_attn_prompt<D>, most, Prompt<D>::kAsk)) return ccuda("kv8_attention: shared memory");
-        k_attn_prompt<D><<<dim3((unsigned) p.tiles, p.c.H, p.n_req), kPromptThreads, Prompt<D>::kAsk, st>>>(p);
-        return ccuda("kv8_attention");
+        const int sm = kAttnWarps * (kTileGroups<D> * 3 * (D / 32) * 256 + 128 + Ring<D>::kBytes);
+        if (!allow_smem(k_attn_tiles<D>, most, sm)) return ccuda("kv8_attention: shared memory");
+        k_attn_tiles<D><<<dim3((unsigned) ((p.tiles + kAttnWarps - 1) / kAttnWarps), p.c.H, p.n_req), kAttnWarps * 32, sm, st>>>(p);
     }
-    static std::atomic<int> most[kMaxDev];
-    const int sm = kAttnWarps * (kTileGroups<D> * 3 * (D / 32) * 256 + 128 + Ring<D>::kBytes);
-    if (!allow_smem(k_attn_tiles<D, SP>, most, sm)) return ccuda("kv8_attention: shared memory");
-    k_attn_tiles<D, SP><<<dim3((unsigned) ((p.tiles + kAttnWarps - 1) / kAttnWarps), p.c.H, p.n_req), kAttnWarps * 32, sm, st>>>(p);
     return ccuda("kv8_attention");
 }
 
@@ -1468,7 +1472,8 @@ int tsb_kv8_attention(const tsb_kv8* cache, const tsb_kv8_attn* d, const void* q
     p.part = (float*) ((uint8_t*) workspace + (((uint64_t) d->n_req + 1) * 8 + 255) / 256 * 256);
     p.wide_out = !((uintptr_t) out % 16 || (d->o_tok * es) % 16 || (d->o_head * es) % 16);
     const int rows = (int) std::min<int64_t>((int64_t) d->max_q * a.G, 1 << 20);
-    const bool two = d->elem_type == E_F32;
+    // the weights in one fp16 value only where the output's rounding is coarser
+    const bool two = d->elem_type != E_BF16;
     cudaStream_t st = cst(stream);
     switch (cache->head_dim) {
         case 64: return two ? launch_attn<64, 2>(p, a, rows, st) : launch_attn<64, 1>(p, a, rows, st);

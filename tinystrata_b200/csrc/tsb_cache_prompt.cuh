@@ -12,7 +12,8 @@
 // memory; its rows are rescaled only when a row's score exceeds its reference by 2^4 (or a block's value scale the
 // largest so far), which after a row's first tiles is rare.
 // Weights are exp2(x - reference + 11), at most 2^15, times the block's value scale relative to the largest so far: fp16 keeps
-// 11 bits of those down to 2^-25 of the reference.  The sums l and everything of the softmax are fp32.
+// 11 bits of those down to 2^-25 of the reference, and for fp16 outputs (LO), whose own rounding is no coarser, a second fp16
+// value holds the rest.  The sums l and everything of the softmax are fp32.
 // What bounds it: at head_dim 256 the products (4 * 128 * 64 * 256 a tile), at 64 the exponentials.
 #pragma once
 
@@ -27,14 +28,14 @@ constexpr unsigned kSitePrompt = 0xC0000001u;   // the error word when a wait of
 constexpr int kPromptThreads = 17 * 32, kConvThreads = 8 * 32, kMmaWarp = 16;
 constexpr float kRefShift = 11.0f, kRefLazy = 4.0f;
 
-template <int D>
+template <int D, bool LO>
 struct Prompt {
-    static constexpr int kN = D == 256 ? 64 : 128;
+    static constexpr int kN = D == 256 || LO ? 64 : 128;
     static constexpr int kQ = 128 * D * 2, kKV = kN * D * 2;
     static constexpr int kGroups = kN / 16;
-    // tensor memory columns: O, S twice, P twice (two weights a column)
-    static constexpr int kS = D, kP = D + 2 * kN;
-    static_assert(kP + kN <= 512, "tensor memory");
+    // tensor memory columns: O, S twice, P twice (two weights a column), with LO the weights' low halves twice
+    static constexpr int kS = D, kP = D + 2 * kN, kLow = kP + kN;
+    static_assert(kP + (LO ? 2 : 1) * kN <= 512, "tensor memory");
     static constexpr int kSmem = kQ + 4 * kKV + 1024;                      // and room to align
     static constexpr int kAsk = kSmem > 120 * 1024 ? kSmem : 120 * 1024;   // one CTA a SM: each takes all of tensor memory
 };
@@ -91,9 +92,9 @@ __device__ __forceinline__ void codes4(uint32_t w, uint32_t& a, uint32_t& b) {
     a = *(const uint32_t*) &u, b = *(const uint32_t*) &v;
 }
 
-template <int D>
+template <int D, bool LO>
 __global__ void __launch_bounds__(kPromptThreads, 1) k_attn_prompt(const __grid_constant__ AttnParams p) {
-    using P = Prompt<D>;
+    using P = Prompt<D, LO>;
     constexpr int N = P::kN, NG = P::kGroups, CH = D / 16;       // CH: 16-code chunks of a token
     extern __shared__ __align__(1024) uint8_t prompt_smem[];
     uint8_t* smem = prompt_smem + ((1024 - (smem_u32(prompt_smem) & 1023)) & 1023);
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_attn_prompt(const __grid_
             const float z = m == -INFINITY ? 0.0f : kRefShift - m;
 #pragma unroll 1
             for (int c0 = NH - 32; c0 >= 0; c0 -= 32) {
-                uint32_t w[16];
+                uint32_t w[16], wl[LO ? 16 : 1];
                 const int ca = half * NH + c0;
                 if (c0 != NH - 32) tm_ld32(from + c0, s);
                 const float sc[2] = {hd[0][ca / 16] * rf, hd[0][ca / 16 + 1] * rf};
@@ -270,9 +271,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_attn_prompt(const __grid_
                     sum = __fadd2_rn(sum, y);
                     const float2 u = __fmul2_rn(y, make_float2(rv[g], rv[g]));
                     w[c / 2] = pack_f16(u.x, u.y);
+                    if constexpr (LO) {
+                        const float2 f = __half22float2(*(const __half2*) &w[c / 2]);
+                        wl[c / 2] = pack_f16(u.x - f.x, u.y - f.y);
+                    }
                 }
                 l += sum.x + sum.y;
                 tm_st16(mine + P::kP + b * (N / 2) + ca / 2, w);
+                if constexpr (LO) tm_st16(mine + P::kLow + b * (N / 2) + ca / 2, wl);
             }
             tm_wait_st();
             tc_fence_before();
@@ -417,6 +423,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_attn_prompt(const __grid_
             const uint32_t from = tmem + P::kP + b * (N / 2);
 #pragma unroll
             for (int k = 0; k < N / 16; ++k) umma_ts(tmem, from + k * 8, vb + ((k * 2048) >> 4), pv, (j | k) != 0);
+            if constexpr (LO) {
+#pragma unroll
+                for (int k = 0; k < N / 16; ++k) umma_ts(tmem, from + (P::kLow - P::kP) + k * 8, vb + ((k * 2048) >> 4), pv, 1);
+            }
             umma_commit(&v_empty[b]);
             umma_commit(&pv_done[b]);
             ++done;
