@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(256) k_kv8_read(const Cache c, const int64_t* 
 // ------------------------------------------------------------------------------------------------ attention
 constexpr int kAttnWarps = 4;
 constexpr int kStep = 16;            // tokens of a step: one matrix-product depth, always within one cache block
-constexpr int kSplitRows = 64, kSplitMost = 1024, kPromptCtas = 24;   // see attn_plan
+constexpr int kSplitRows = 64, kPromptCtas = 12, kPromptCtas32 = 40;   // see attn_plan
 constexpr int kMaxReq = 4096;
 
 struct AttnParams {
@@ -1309,10 +1309,13 @@ int attn_plan(const tsb_kv8* c, const tsb_kv8_attn* d, AttnPlan& a) {
     const int64_t rows = (int64_t) d->max_q * a.G;
     if (rows > (1 << 28)) return cfail(TSB_ERR_UNSUPPORTED, "kv8_attention: too many query rows");
     // Rows a key / value head has (queries x heads of its group).  Up to 64 the steps of a request are split over CTAs; above,
-    // tiles of rows walk all of their keys, 16-bit queries in tiles of 128 on tcgen05.  A few hundred rows whose tiles would
-    // leave most SMs idle are split too.
+    // tiles of rows walk all of their keys, 16-bit queries in tiles of 128 on tcgen05.  More rows are split too while their
+    // tiles would leave most SMs idle.  Measured, split against tiles (us): 64 rows, 16 requests of 2000 keys, 41 against 49
+    // (fp32 43 against 212); 128 rows of them 60 against 54; 512 rows in 8 tiles, 3000 keys of 256, 58 against 102; 768 rows in
+    // 12 tiles, 2000 keys, 54 against 54; 512 rows in 16, 128 keys, 40 against 23.  The fp32 tiles are smaller and slower:
+    // 1536 rows in 24 tiles, 3000 keys, 101 against 303; 4096 in 32, 2000 keys, 174 against 210; 6744 in 53 293 against 209.
     const int64_t prompt_ctas = (rows + 127) / 128 * c->n_kv_heads * d->n_req;
-    a.split = rows <= kSplitRows || (rows <= kSplitMost && prompt_ctas < kPromptCtas);
+    a.split = rows <= kSplitRows || prompt_ctas < (d->elem_type == E_F32 ? kPromptCtas32 : kPromptCtas);
     a.prompt = !a.split && d->elem_type != E_F32;
     a.groups = a.prompt ? 16 : !a.split ? (c->head_dim == 256 ? kTileGroups<256> : kTileGroups<128>) : rows <= 8 ? 1 : 2;
     a.tiles = (int) ((rows + 8 * a.groups - 1) / (8 * a.groups));

@@ -608,11 +608,12 @@ __global__ void __launch_bounds__(128, E == E_F32 ? 2 : 4) k_delta_prepare(const
     }
 }
 
-// The W warps that share 16 value columns.
-template <int W>
-__device__ __forceinline__ void unit_sync(int unit) {
-    if constexpr (W > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + unit), "n"(32 * W) : "memory");
-}
+// Barriers of the warps that share 16 value columns (two units a CTA): the two that carry the state; those and the two that
+// write the outputs; and the latter's word to the former that they have read the state.
+__device__ __forceinline__ void pair_sync(int unit) { asm volatile("bar.sync %0, 64;" ::"r"(1 + unit) : "memory"); }
+__device__ __forceinline__ void unit_sync(int unit) { asm volatile("bar.sync %0, 128;" ::"r"(3 + unit) : "memory"); }
+__device__ __forceinline__ void read_sync(int unit) { asm volatile("bar.sync %0, 128;" ::"r"(5 + unit) : "memory"); }
+__device__ __forceinline__ void read_arrive(int unit) { asm volatile("bar.arrive %0, 128;" ::"r"(5 + unit) : "memory"); }
 
 // The power-of-two scales of a left operand's rows g and g + 8, and their inverses: largest magnitudes in [2^9, 2^10), so
 // that the next chunk's may grow 32-fold.
@@ -637,12 +638,13 @@ struct RowScale {
 // whose right operands are the chunk's tiles (bulk copies, two chunks deep).  W 1: a warp owns its unit and exchanges
 // nothing, eight units a CTA; W 2: the warps take half of every product's columns (tokens, keys) each and pass the left
 // operands through shared memory, two units a CTA; operands are written under the scales of the chunk before, and again
-// in the rare case that a row outgrew them, so that an exchange is one barrier.  What bounds it: a sequence's chunks
+// in the rare case that a row outgrew them, so that an exchange is one barrier.  Two more warps a unit (the writers) take
+// Z and O, which no later chunk waits for, from the same exchanges.  What bounds it: a sequence's chunks
 // follow one another, and a unit's 400 products of 16 x 8 x 16 a chunk (bf16, dim_k 128) at 8 cycles each.  One sequence
 // of 32 heads has 256 units, so W 2 puts them on 128 SMs with every scheduler at work; with more sequences W 1 does the
 // same work without exchanges.
 template <int E, int DK, int W>
-__global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaParams p) {
+__global__ void __launch_bounds__(256) k_delta_scan(const DeltaParams p) {
     using T = Tiles<E, DK>;
     constexpr int PL = T::PL;
     constexpr bool OS = T::PP == 2;
@@ -656,7 +658,8 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaPa
     __shared__ int sh[8];
     __shared__ float peaks[UN][4][W][16];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, qd = lane & 3;
-    const int unit = warp / W, part = warp % W;
+    const bool writer = W == 2 && warp >= 4;           // W 2: warps 0-3 carry the states of two units, 4-7 write the outputs
+    const int unit = (warp & (UN * W - 1)) / W, part = warp % W;
     const int h = blockIdx.y, b = blockIdx.z, hk = h / (p.hv / p.hk);
     const Seq s = seq_of(p, b);
     const int st = state_of(p, b);
@@ -669,7 +672,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaPa
     uint4* fu = fs + 256;                                       // U [4][2][32]
     uint4* fx = fs + 512;                                       // X [4][2][32]
     if (tid == 0) {
-        for (int i = 0; i < 2; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], UN * W);
+        for (int i = 0; i < 2; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 8);
         fence_mbar_init();
     }
     __syncthreads();
@@ -681,7 +684,8 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaPa
         bulk_g2s(sm + i * T::kStage, src + (int64_t) hk * T::kHead, T::kHead, &full[i]);
         bulk_g2s(sm + i * T::kStage + T::kHead, src + (int64_t) p.hk * T::kHead + (int64_t) h * T::kVal, T::kVal, &full[i]);
     };
-    if (tid == 0) {
+    const bool fetches = tid == (W == 1 ? 0 : 128);
+    if (fetches) {
         for (int c = 0; c < min(chunks, 2); ++c) fetch(c);
     }
     // a warp's token tiles: with two warps 0, 3 and 1, 2, which share the triangles' work evenly
@@ -692,7 +696,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaPa
     for (int i = 0; i < NK; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            S[i][e] = st >= 0 && in ? p.s_in[base + (int64_t) (i * 8 + 2 * qd + (e & 1)) * p.dv + g + (e >> 1) * 8] : 0.0f;
+            S[i][e] = st >= 0 && in && !writer ? p.s_in[base + (int64_t) (i * 8 + 2 * qd + (e & 1)) * p.dv + g + (e >> 1) * 8] : 0.0f;
 
     auto split_a = [&](const float (&x)[4], const float (&y)[4], const RowScale& r, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
         split_f16x2(x[0], x[1], r.u[0], hi[0], lo[0]);
@@ -744,13 +748,13 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaPa
             rs.set(a, c);
         } else {
             put_state();
-            unit_sync<W>(unit);
+            unit_sync(unit);
             join_peak(a, c, 0);
             if (!__all_sync(0xffffffffu, rs.holds(a, c))) {      // the same in every warp of the unit
                 rs.set(a, c);
-                unit_sync<W>(unit);
+                unit_sync(unit);
                 put_state();
-                unit_sync<W>(unit);
+                unit_sync(unit);
             }
         }
     };
@@ -779,18 +783,147 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaPa
         else if constexpr (E == E_F16) return __half2float(__ushort_as_half(r));
         else return __uint_as_float((uint32_t) r << 16);
     };
-    if (chunks > 0) load_values(0);
-    share_state();
-
     // byte offsets of a lane's ldmatrix rows: right operands by rows (16 tokens a load) and transposed (keys); the
     // piece of depth d or key tile n is an xor with 32 d or 32 n
     const int br = (lane & 7) + (lane >> 4) * 8, tr = (lane & 7) + ((lane >> 3) & 1) * 8;
     const uint32_t row_x = (((lane >> 3) & 1) ^ (br & 7)) << 4, col_x = ((lane >> 4) ^ (tr & 7)) << 4;
     bool ok = true;
+    // a chunk's tiles are read by all 8 warps; then those of the chunk after the next take their place
+    auto release = [&](int c) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[c & 1]);
+        if (fetches && c + 2 < chunks && ok) {
+            ok = mbar_wait_bounded(&empty[c & 1], (c >> 1) & 1, p.err, kSiteDelta);
+            if (ok) fetch(c + 2);
+        }
+    };
+    // Z^T: tokens' states' part of the outputs
+    auto scale_z = [&](float (&Z)[NP * 2][4], const float* vec) {
+#pragma unroll
+        for (int n = 0; n < NP * 2; ++n) {
+            const float2 eq = *(const float2*) (vec + V_EQ + tile_of(n >> 1) * 16 + (n & 1) * 8 + 2 * qd);
+            Z[n][0] *= eq.x * rs.i[0], Z[n][1] *= eq.y * rs.i[0], Z[n][2] *= eq.x * rs.i[1], Z[n][3] *= eq.y * rs.i[1];
+        }
+    };
+    // O^T = Z^T + U^T P^T of chunk c, from U's left operands
+    auto outputs = [&](int c, uint32_t mr, const float* vec, const float (&Z)[NP * 2][4], const uint32_t (&xh)[4][4], const uint32_t (&xl)[4][4]) {
+        const int live = in ? min(kChunk, s.n - c * kChunk) : 0;
+        float O[NP * 2][4];
+#pragma unroll
+        for (int n = 0; n < NP * 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) O[n][e] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            const uint32_t at = mr + (row_x ^ (32 * d)) + 2 * T::kSq;
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                if (d > tile_of(n)) continue;
+                uint32_t r[4];
+                ldsm4(r, at + tile_of(n) * 16 * SB);
+                mma_f16(O[2 * n], xh[d], r[0], r[1]);
+                mma_f16(O[2 * n + 1], xh[d], r[2], r[3]);
+                if (OS) {
+                    uint32_t w[4];
+                    ldsm4(w, at + tile_of(n) * 16 * SB + T::kSq);
+                    mma_f16(O[2 * n], xl[d], r[0], r[1]);
+                    mma_f16(O[2 * n + 1], xl[d], r[2], r[3]);
+                    mma_f16(O[2 * n], xh[d], w[0], w[1]);
+                    mma_f16(O[2 * n + 1], xh[d], w[2], w[3]);
+                }
+            }
+        }
+        Out* r0 = op + (s.tok + (int64_t) c * kChunk + 2 * qd) * p.o_tok;
+#pragma unroll
+        for (int n = 0; n < NP * 2; ++n) {
+            const int t0 = tile_of(n >> 1) * 16 + (n & 1) * 8;
+            const float2 fp = *(const float2*) (vec + V_FP + t0 + 2 * qd);
+            Out* r = r0 + t0 * p.o_tok;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float o = fmaf(O[n][e], (e & 1 ? fp.y : fp.x) * ru.i[e >> 1], Z[n][e]);
+                Out* at = (e & 1 ? r + p.o_tok : r) + (e >> 1) * 8;
+                if (t0 + 2 * qd + (e & 1) < live) store_t<E>(at, o);
+            }
+        }
+    };
+    auto in_flight = [&]() {                    // after a wait that gave up: copies land before the CTA's memory goes
+        for (int i = 0; i < 2; ++i)
+            for (int ph = 0; ph < 2; ++ph) mbar_wait_bounded(&full[i], ph, p.err, kSiteDelta);
+    };
+    if constexpr (W == 2) {
+        if (writer) {                           // meets the same barriers as the warps that carry the states, and knows their scales
+            auto meet_state = [&]() {
+                float a = 0.0f, cc = 0.0f;
+                unit_sync(unit);
+                join_peak(a, cc, 0);
+                if (!__all_sync(0xffffffffu, rs.holds(a, cc))) {
+                    rs.set(a, cc);
+                    unit_sync(unit);
+                    unit_sync(unit);
+                }
+            };
+            meet_state();
+            for (int c = 0; c < chunks; ++c) {
+                const int i = c & 1;
+                if (ok) ok = mbar_wait_bounded(&full[i], (c >> 1) & 1, p.err, kSiteDelta);
+                const uint32_t kt = smem_u32(sm + i * T::kStage), mt = kt + T::kHead;
+                const float* vec = (const float*) (sm + i * T::kStage + T::kHead + (2 + T::PP) * T::kSq);
+                float Z[NP * 2][4];
+#pragma unroll
+                for (int n = 0; n < NP * 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) Z[n][e] = 0.0f;
+#pragma unroll
+                for (int d = 0; d < DK / 16; ++d) {
+                    uint32_t hi[4], lo[4], rq[NP][PL][4];
+#pragma unroll
+                    for (int n = 0; n < NP; ++n)
+#pragma unroll
+                        for (int l = 0; l < PL; ++l) ldsm4(rq[n][l], kt + br * RB + (row_x ^ (32 * d)) + tile_of(n) * 16 * RB + (PL + l) * T::kTile);
+                    get(fs, d, hi, lo);
+#pragma unroll
+                    for (int l = 0; l < PL; ++l)
+#pragma unroll
+                        for (int n = 0; n < NP; ++n) {
+                            mma_f16(Z[2 * n], hi, rq[n][l][0], rq[n][l][1]);
+                            mma_f16(Z[2 * n + 1], hi, rq[n][l][2], rq[n][l][3]);
+                        }
+                    if (OS) {
+#pragma unroll
+                        for (int n = 0; n < NP; ++n) {
+                            mma_f16(Z[2 * n], lo, rq[n][0][0], rq[n][0][1]);
+                            mma_f16(Z[2 * n + 1], lo, rq[n][0][2], rq[n][0][3]);
+                        }
+                    }
+                }
+                scale_z(Z, vec);
+                read_arrive(unit);
+                float ua = 0.0f, uc = 0.0f, fa = 0.0f, fc = 0.0f;
+                unit_sync(unit);
+                join_peak(ua, uc, 2);
+                join_peak(fa, fc, 3);
+                if (!__all_sync(0xffffffffu, ru.holds(ua, uc) && rf.holds(fa, fc))) {
+                    ru.set(ua, uc);
+                    rf.set(fa, fc);
+                    unit_sync(unit);
+                    unit_sync(unit);
+                }
+                uint32_t xh[4][4], xl[4][4];
+#pragma unroll
+                for (int d = 0; d < 4; ++d) get(fu, d, xh[d], xl[d]);
+                outputs(c, mt + br * SB, vec, Z, xh, xl);
+                release(c);
+                if (c + 1 < chunks) meet_state();
+            }
+            if (!ok) in_flight();
+            return;
+        }
+    }
+    if (chunks > 0) load_values(0);
+    share_state();
     for (int c = 0; c < chunks; ++c) {
         const int i = c & 1;
-        const int64_t tok0 = s.tok + (int64_t) c * kChunk;
-        const int live = in ? min(kChunk, s.n - c * kChunk) : 0;
         // after a wait that gave up the loop runs on over whatever the tiles hold, so that every barrier is met
         if (ok) ok = mbar_wait_bounded(&full[i], (c >> 1) & 1, p.err, kSiteDelta);
         const uint32_t kt = smem_u32(sm + i * T::kStage), mt = kt + T::kHead;
@@ -811,7 +944,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaPa
 #pragma unroll
                 for (int l = 0; l < PL; ++l) {
                     ldsm4(rk[n][l], at + tile_of(n) * 16 * RB + l * T::kTile);
-                    ldsm4(rq[n][l], at + tile_of(n) * 16 * RB + (PL + l) * T::kTile);
+                    if (W == 1) ldsm4(rq[n][l], at + tile_of(n) * 16 * RB + (PL + l) * T::kTile);
                 }
             if constexpr (W == 1) split_a(S[2 * d], S[2 * d + 1], rs, hi, lo);
             else get(fs, d, hi, lo);
@@ -821,27 +954,29 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaPa
                 for (int n = 0; n < NP; ++n) {
                     mma_f16(Y[2 * n], hi, rk[n][l][0], rk[n][l][1]);
                     mma_f16(Y[2 * n + 1], hi, rk[n][l][2], rk[n][l][3]);
-                    mma_f16(Z[2 * n], hi, rq[n][l][0], rq[n][l][1]);
-                    mma_f16(Z[2 * n + 1], hi, rq[n][l][2], rq[n][l][3]);
+                    if (W == 1) {
+                        mma_f16(Z[2 * n], hi, rq[n][l][0], rq[n][l][1]);
+                        mma_f16(Z[2 * n + 1], hi, rq[n][l][2], rq[n][l][3]);
+                    }
                 }
 #pragma unroll
             for (int n = 0; n < NP; ++n) {
                 mma_f16(Y[2 * n], lo, rk[n][0][0], rk[n][0][1]);
                 mma_f16(Y[2 * n + 1], lo, rk[n][0][2], rk[n][0][3]);
-                if (OS) {
+                if (W == 1 && OS) {
                     mma_f16(Z[2 * n], lo, rq[n][0][0], rq[n][0][1]);
                     mma_f16(Z[2 * n + 1], lo, rq[n][0][2], rq[n][0][3]);
                 }
             }
         }
+        if (W == 1) scale_z(Z, vec);
         float a = 0.0f, cc = 0.0f;
 #pragma unroll
         for (int n = 0; n < NP * 2; ++n) {
             const int t = tile_of(n >> 1) * 16 + (n & 1) * 8 + 2 * qd;
-            const float2 ek = *(const float2*) (vec + V_EK + t), eq = *(const float2*) (vec + V_EQ + t);
+            const float2 ek = *(const float2*) (vec + V_EK + t);
             Y[n][0] = fmaf(-ek.x * rs.i[0], Y[n][0], value(V[n][0])), Y[n][1] = fmaf(-ek.y * rs.i[0], Y[n][1], value(V[n][1]));
             Y[n][2] = fmaf(-ek.x * rs.i[1], Y[n][2], value(V[n][2])), Y[n][3] = fmaf(-ek.y * rs.i[1], Y[n][3], value(V[n][3]));
-            Z[n][0] *= eq.x * rs.i[0], Z[n][1] *= eq.y * rs.i[0], Z[n][2] *= eq.x * rs.i[1], Z[n][3] *= eq.y * rs.i[1];
             a = fmaxf(a, fmaxf(fabsf(Y[n][0]), fabsf(Y[n][1])));
             cc = fmaxf(cc, fmaxf(fabsf(Y[n][2]), fabsf(Y[n][3])));
         }
@@ -856,14 +991,14 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaPa
         } else {
 #pragma unroll
             for (int n = 0; n < NP; ++n) put(fx, tile_of(n), Y[2 * n], Y[2 * n + 1], rx);
-            unit_sync<W>(unit);
+            pair_sync(unit);
             join_peak(a, cc, 1);
             if (!__all_sync(0xffffffffu, rx.holds(a, cc))) {
                 rx.set(a, cc);
-                unit_sync<W>(unit);
+                pair_sync(unit);
 #pragma unroll
                 for (int n = 0; n < NP; ++n) put(fx, tile_of(n), Y[2 * n], Y[2 * n + 1], rx);
-                unit_sync<W>(unit);
+                pair_sync(unit);
             }
 #pragma unroll
             for (int d = 0; d < 4; ++d) get(fx, d, xh[d], xl[d]);
@@ -922,22 +1057,20 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaPa
                     put(fs, tile_of(n), F[2 * n], F[2 * n + 1], rf);
                 }
             };
+            read_sync(unit);                        // the writers have read S and the last chunk's U
             put_u();
-            unit_sync<W>(unit);
+            unit_sync(unit);
             join_peak(ua, uc, 2);
             join_peak(fa, fc, 3);
             if (!__all_sync(0xffffffffu, ru.holds(ua, uc) && rf.holds(fa, fc))) {
                 ru.set(ua, uc);
                 rf.set(fa, fc);
-                unit_sync<W>(unit);
+                unit_sync(unit);
                 put_u();
-                unit_sync<W>(unit);
+                unit_sync(unit);
             }
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                get(fs, d, fh[d], fl[d]);
-                get(fu, d, xh[d], xl[d]);
-            }
+            for (int d = 0; d < 4; ++d) get(fs, d, fh[d], fl[d]);
         }
         // S^T, two pairs of key tiles at a time (eight products in flight): the scaled product is added in fp32
         const float end = vec[V_END];
@@ -971,61 +1104,15 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 128) k_delta_scan(const DeltaPa
 #pragma unroll
                 for (int e = 0; e < 4; ++e) S[2 * n + x][e] = fmaf(acc[x][e], end_f[e >> 1], S[2 * n + x][e] * end);
         }
-        // O^T
-        float O[NP * 2][4];
-#pragma unroll
-        for (int n = 0; n < NP * 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) O[n][e] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            const uint32_t at = mr + (row_x ^ (32 * d)) + 2 * T::kSq;
-#pragma unroll
-            for (int n = 0; n < NP; ++n) {
-                if (d > tile_of(n)) continue;
-                uint32_t r[4];
-                ldsm4(r, at + tile_of(n) * 16 * SB);
-                mma_f16(O[2 * n], xh[d], r[0], r[1]);
-                mma_f16(O[2 * n + 1], xh[d], r[2], r[3]);
-                if (OS) {
-                    uint32_t w[4];
-                    ldsm4(w, at + tile_of(n) * 16 * SB + T::kSq);
-                    mma_f16(O[2 * n], xl[d], r[0], r[1]);
-                    mma_f16(O[2 * n + 1], xl[d], r[2], r[3]);
-                    mma_f16(O[2 * n], xh[d], w[0], w[1]);
-                    mma_f16(O[2 * n + 1], xh[d], w[2], w[3]);
-                }
-            }
-        }
-        {
-            Out* r0 = op + (tok0 + 2 * qd) * p.o_tok;
-#pragma unroll
-            for (int n = 0; n < NP * 2; ++n) {
-                const int t0 = tile_of(n >> 1) * 16 + (n & 1) * 8;
-                const float2 fp = *(const float2*) (vec + V_FP + t0 + 2 * qd);
-                Out* r = r0 + t0 * p.o_tok;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float o = fmaf(O[n][e], (e & 1 ? fp.y : fp.x) * ru.i[e >> 1], Z[n][e]);
-                    Out* at = (e & 1 ? r + p.o_tok : r) + (e >> 1) * 8;
-                    if (t0 + 2 * qd + (e & 1) < live) store_t<E>(at, o);
-                }
-            }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[i]);
-        if (tid == 0 && c + 2 < chunks && ok) {
-            ok = mbar_wait_bounded(&empty[i], (c >> 1) & 1, p.err, kSiteDelta);
-            if (ok) fetch(c + 2);
-        }
+        if (W == 1) outputs(c, mr, vec, Z, xh, xl);
+        release(c);
         if (c + 1 < chunks) {
-            unit_sync<W>(unit);                     // the exchange is read
+            if (W == 2) pair_sync(unit);            // F is read
             share_state();
         }
     }
-    if (!ok) {                                  // let copies in flight land before the CTA's memory goes
-        for (int i = 0; i < 2; ++i)
-            for (int ph = 0; ph < 2; ++ph) mbar_wait_bounded(&full[i], ph, p.err, kSiteDelta);
+    if (!ok) {
+        in_flight();
         return;
     }
     if (st >= 0 && in) {
@@ -1071,7 +1158,7 @@ int launch_scan(const DeltaParams& p, cudaStream_t st) {
     static_assert(sm <= 226 * 1024, "shared memory");
     if (cudaFuncSetAttribute(k_delta_scan<E, DK, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm) != cudaSuccess)
         return dcuda("gated_delta: shared memory");
-    k_delta_scan<E, DK, W><<<dim3((unsigned) ((p.dv + 16 * un - 1) / (16 * un)), p.hv, p.n_seq), un * W * 32, sm, st>>>(p);
+    k_delta_scan<E, DK, W><<<dim3((unsigned) ((p.dv + 16 * un - 1) / (16 * un)), p.hv, p.n_seq), 256, sm, st>>>(p);
     return dcuda("gated_delta");
 }
 template <int E, int DK>
