@@ -612,6 +612,16 @@ __global__ void __launch_bounds__(128, E == E_F32 ? 2 : 4) k_delta_prepare(const
 // write the outputs; and the latter's word to the former that they have read the state.
 __device__ __forceinline__ void pair_sync(int unit) { asm volatile("bar.sync %0, 64;" ::"r"(1 + unit) : "memory"); }
 __device__ __forceinline__ void unit_sync(int unit) { asm volatile("bar.sync %0, 128;" ::"r"(3 + unit) : "memory"); }
+// The same barriers, and whether any of their threads says so.
+template <int N>
+__device__ __forceinline__ bool sync_any(int id, bool x) {
+    uint32_t r;
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 q, %2, 0;\n bar.red.or.pred p, %1, %3, q;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(r) : "r"(id), "r"((uint32_t) x), "n"(N) : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ bool pair_any(int unit, bool x) { return sync_any<64>(1 + unit, x); }
+__device__ __forceinline__ bool unit_any(int unit, bool x) { return sync_any<128>(3 + unit, x); }
 __device__ __forceinline__ void read_sync(int unit) { asm volatile("bar.sync %0, 128;" ::"r"(5 + unit) : "memory"); }
 __device__ __forceinline__ void read_arrive(int unit) { asm volatile("bar.arrive %0, 128;" ::"r"(5 + unit) : "memory"); }
 
@@ -624,7 +634,7 @@ struct RowScale {
         pow2_scale(c, u[1], i[1]);
         u[0] *= 0.03125f, u[1] *= 0.03125f, i[0] *= 32.0f, i[1] *= 32.0f;
     }
-    // Whether rows with these largest magnitudes fit fp16 pairs under the scales at full accuracy: at most 2^15, and not
+    // Whether rows (or one lane's part of them) with these largest magnitudes fit fp16 pairs under the scales at full accuracy: at most 2^15, and not
     // so small that the low halves (multiples of 2^-24) lose bits.
     __device__ __forceinline__ bool holds(float a, float c) const {
         const float x = a * u[0], y = c * u[1];
@@ -639,7 +649,7 @@ struct RowScale {
 // nothing, eight units a CTA; W 2: the warps take half of every product's columns (tokens, keys) each and pass the left
 // operands through shared memory, two units a CTA; operands are written under the scales of the chunk before, and again
 // in the rare case that a row outgrew them, so that an exchange is one barrier.  Two more warps a unit (the writers) take
-// Z and O, which no later chunk waits for, from the same exchanges.  What bounds it: a sequence's chunks
+// Z and O, which no later chunk waits for, from the same exchanges, and bring V.  What bounds it: a sequence's chunks
 // follow one another, and a unit's 400 products of 16 x 8 x 16 a chunk (bf16, dim_k 128) at 8 cycles each.  One sequence
 // of 32 heads has 256 units, so W 2 puts them on 128 SMs with every scheduler at work; with more sequences W 1 does the
 // same work without exchanges.
@@ -743,16 +753,16 @@ __global__ void __launch_bounds__(256) k_delta_scan(const DeltaParams p) {
     auto share_state = [&]() {
         float a, c;
         state_peak(a, c);
-        tell_peak(a, c, 0);
         if constexpr (W == 1) {
+            tell_peak(a, c, 0);
             rs.set(a, c);
         } else {
             put_state();
-            unit_sync(unit);
-            join_peak(a, c, 0);
-            if (!__all_sync(0xffffffffu, rs.holds(a, c))) {      // the same in every warp of the unit
-                rs.set(a, c);
+            if (unit_any(unit, !rs.holds(a, c))) {
+                tell_peak(a, c, 0);
                 unit_sync(unit);
+                join_peak(a, c, 0);
+                rs.set(a, c);
                 put_state();
                 unit_sync(unit);
             }
@@ -854,18 +864,29 @@ __global__ void __launch_bounds__(256) k_delta_scan(const DeltaParams p) {
     if constexpr (W == 2) {
         if (writer) {                           // meets the same barriers as the warps that carry the states, and knows their scales
             auto meet_state = [&]() {
-                float a = 0.0f, cc = 0.0f;
-                unit_sync(unit);
-                join_peak(a, cc, 0);
-                if (!__all_sync(0xffffffffu, rs.holds(a, cc))) {
-                    rs.set(a, cc);
+                if (unit_any(unit, false)) {
+                    float a = 0.0f, cc = 0.0f;
                     unit_sync(unit);
+                    join_peak(a, cc, 0);
+                    rs.set(a, cc);
                     unit_sync(unit);
                 }
             };
+            // the next chunk's values to the warps that carry the states: each lane's own, where it will put its X
+            auto give_values = [&]() {
+#pragma unroll
+                for (int n = 0; n < NP * 2; ++n)
+                    ((float4*) fx)[(tile_of(n >> 1) * 2 + (n & 1)) * 32 + lane] =
+                        make_float4(value(V[n][0]), value(V[n][1]), value(V[n][2]), value(V[n][3]));
+            };
+            if (chunks > 0) {
+                load_values(0);
+                give_values();
+            }
             meet_state();
             for (int c = 0; c < chunks; ++c) {
                 const int i = c & 1;
+                if (c + 1 < chunks) load_values(c + 1);
                 if (ok) ok = mbar_wait_bounded(&full[i], (c >> 1) & 1, p.err, kSiteDelta);
                 const uint32_t kt = smem_u32(sm + i * T::kStage), mt = kt + T::kHead;
                 const float* vec = (const float*) (sm + i * T::kStage + T::kHead + (2 + T::PP) * T::kSq);
@@ -899,16 +920,14 @@ __global__ void __launch_bounds__(256) k_delta_scan(const DeltaParams p) {
                 }
                 scale_z(Z, vec);
                 read_arrive(unit);
-                float ua = 0.0f, uc = 0.0f, fa = 0.0f, fc = 0.0f;
-                unit_sync(unit);
-                join_peak(ua, uc, 2);
-                join_peak(fa, fc, 3);
-                if (!__all_sync(0xffffffffu, ru.holds(ua, uc) && rf.holds(fa, fc))) {
-                    ru.set(ua, uc);
-                    rf.set(fa, fc);
+                if (unit_any(unit, false)) {
+                    float a = 0.0f, cc = 0.0f;
                     unit_sync(unit);
+                    join_peak(a, cc, 2);
+                    ru.set(a, cc);
                     unit_sync(unit);
                 }
+                if (c + 1 < chunks) give_values();
                 uint32_t xh[4][4], xl[4][4];
 #pragma unroll
                 for (int d = 0; d < 4; ++d) get(fu, d, xh[d], xl[d]);
@@ -920,7 +939,7 @@ __global__ void __launch_bounds__(256) k_delta_scan(const DeltaParams p) {
             return;
         }
     }
-    if (chunks > 0) load_values(0);
+    if (W == 1 && chunks > 0) load_values(0);
     share_state();
     for (int c = 0; c < chunks; ++c) {
         const int i = c & 1;
@@ -975,27 +994,30 @@ __global__ void __launch_bounds__(256) k_delta_scan(const DeltaParams p) {
         for (int n = 0; n < NP * 2; ++n) {
             const int t = tile_of(n >> 1) * 16 + (n & 1) * 8 + 2 * qd;
             const float2 ek = *(const float2*) (vec + V_EK + t);
-            Y[n][0] = fmaf(-ek.x * rs.i[0], Y[n][0], value(V[n][0])), Y[n][1] = fmaf(-ek.y * rs.i[0], Y[n][1], value(V[n][1]));
-            Y[n][2] = fmaf(-ek.x * rs.i[1], Y[n][2], value(V[n][2])), Y[n][3] = fmaf(-ek.y * rs.i[1], Y[n][3], value(V[n][3]));
+            float4 v;
+            if constexpr (W == 1) v = make_float4(value(V[n][0]), value(V[n][1]), value(V[n][2]), value(V[n][3]));
+            else v = ((const float4*) fx)[(tile_of(n >> 1) * 2 + (n & 1)) * 32 + lane];
+            Y[n][0] = fmaf(-ek.x * rs.i[0], Y[n][0], v.x), Y[n][1] = fmaf(-ek.y * rs.i[0], Y[n][1], v.y);
+            Y[n][2] = fmaf(-ek.x * rs.i[1], Y[n][2], v.z), Y[n][3] = fmaf(-ek.y * rs.i[1], Y[n][3], v.w);
             a = fmaxf(a, fmaxf(fabsf(Y[n][0]), fabsf(Y[n][1])));
             cc = fmaxf(cc, fmaxf(fabsf(Y[n][2]), fabsf(Y[n][3])));
         }
-        if (c + 1 < chunks) load_values(c + 1);   // they arrive during the rest of this chunk
+        if (W == 1 && c + 1 < chunks) load_values(c + 1);   // they arrive during the rest of this chunk
 
         uint32_t xh[4][4], xl[4][4];               // X's left operands, all token tiles; then U's
-        tell_peak(a, cc, 1);
         if constexpr (W == 1) {
+            tell_peak(a, cc, 1);
             rx.set(a, cc);
 #pragma unroll
             for (int d = 0; d < 4; ++d) split_a(Y[2 * d], Y[2 * d + 1], rx, xh[d], xl[d]);
         } else {
 #pragma unroll
             for (int n = 0; n < NP; ++n) put(fx, tile_of(n), Y[2 * n], Y[2 * n + 1], rx);
-            pair_sync(unit);
-            join_peak(a, cc, 1);
-            if (!__all_sync(0xffffffffu, rx.holds(a, cc))) {
-                rx.set(a, cc);
+            if (pair_any(unit, !rx.holds(a, cc))) {
+                tell_peak(a, cc, 1);
                 pair_sync(unit);
+                join_peak(a, cc, 1);
+                rx.set(a, cc);
 #pragma unroll
                 for (int n = 0; n < NP; ++n) put(fx, tile_of(n), Y[2 * n], Y[2 * n + 1], rx);
                 pair_sync(unit);
@@ -1039,9 +1061,9 @@ __global__ void __launch_bounds__(256) k_delta_scan(const DeltaParams p) {
             fa = fmaxf(fa, fmaxf(fabsf(F[n][0]), fabsf(F[n][1]))), fc = fmaxf(fc, fmaxf(fabsf(F[n][2]), fabsf(F[n][3])));
         }
         uint32_t fh[4][4], fl[4][4];
-        tell_peak(ua, uc, 2);
-        tell_peak(fa, fc, 3);
         if constexpr (W == 1) {
+            tell_peak(ua, uc, 2);
+            tell_peak(fa, fc, 3);
             ru.set(ua, uc);
             rf.set(fa, fc);
 #pragma unroll
@@ -1059,13 +1081,14 @@ __global__ void __launch_bounds__(256) k_delta_scan(const DeltaParams p) {
             };
             read_sync(unit);                        // the writers have read S and the last chunk's U
             put_u();
-            unit_sync(unit);
-            join_peak(ua, uc, 2);
-            join_peak(fa, fc, 3);
-            if (!__all_sync(0xffffffffu, ru.holds(ua, uc) && rf.holds(fa, fc))) {
+            if (unit_any(unit, !(ru.holds(ua, uc) && rf.holds(fa, fc)))) {
+                tell_peak(ua, uc, 2);
+                tell_peak(fa, fc, 3);
+                unit_sync(unit);
+                join_peak(ua, uc, 2);
+                join_peak(fa, fc, 3);
                 ru.set(ua, uc);
                 rf.set(fa, fc);
-                unit_sync(unit);
                 put_u();
                 unit_sync(unit);
             }
