@@ -920,11 +920,14 @@ __global__ void __launch_bounds__(256) k_delta_scan(const DeltaParams p) {
                 }
                 scale_z(Z, vec);
                 read_arrive(unit);
-                if (unit_any(unit, false)) {
-                    float a = 0.0f, cc = 0.0f;
+                float ua = 0.0f, uc = 0.0f, fa = 0.0f, fc = 0.0f;
+                unit_sync(unit);
+                join_peak(ua, uc, 2);
+                join_peak(fa, fc, 3);
+                if (!__all_sync(0xffffffffu, ru.holds(ua, uc) && rf.holds(fa, fc))) {
+                    ru.set(ua, uc);
+                    rf.set(fa, fc);
                     unit_sync(unit);
-                    join_peak(a, cc, 2);
-                    ru.set(a, cc);
                     unit_sync(unit);
                 }
                 if (c + 1 < chunks) give_values();
@@ -1061,9 +1064,9 @@ __global__ void __launch_bounds__(256) k_delta_scan(const DeltaParams p) {
             fa = fmaxf(fa, fmaxf(fabsf(F[n][0]), fabsf(F[n][1]))), fc = fmaxf(fc, fmaxf(fabsf(F[n][2]), fabsf(F[n][3])));
         }
         uint32_t fh[4][4], fl[4][4];
+        tell_peak(ua, uc, 2);
+        tell_peak(fa, fc, 3);
         if constexpr (W == 1) {
-            tell_peak(ua, uc, 2);
-            tell_peak(fa, fc, 3);
             ru.set(ua, uc);
             rf.set(fa, fc);
 #pragma unroll
@@ -1081,14 +1084,14 @@ __global__ void __launch_bounds__(256) k_delta_scan(const DeltaParams p) {
             };
             read_sync(unit);                        // the writers have read S and the last chunk's U
             put_u();
-            if (unit_any(unit, !(ru.holds(ua, uc) && rf.holds(fa, fc)))) {
-                tell_peak(ua, uc, 2);
-                tell_peak(fa, fc, 3);
-                unit_sync(unit);
-                join_peak(ua, uc, 2);
-                join_peak(fa, fc, 3);
+            // (by the rows' own peaks: the decay leaves most lanes of F far below theirs)
+            unit_sync(unit);
+            join_peak(ua, uc, 2);
+            join_peak(fa, fc, 3);
+            if (!__all_sync(0xffffffffu, ru.holds(ua, uc) && rf.holds(fa, fc))) {
                 ru.set(ua, uc);
                 rf.set(fa, fc);
+                unit_sync(unit);
                 put_u();
                 unit_sync(unit);
             }
