@@ -231,6 +231,16 @@ def test_attention_prompts(T, dtype, queries, lens, window, H, G, D, bs):
     _attend(T, np.random.default_rng(11), lens, queries, H, G, D, bs, dtype, window)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("queries,lens,window,H,G,D,bs", [
+    ([300, 300, 299], [300, 299, 450], 0, 5, 2, 64, 16), ([129, 70, 400], [500, 70, 400], 0, 4, 4, 128, 32),
+    ([33, 90], [1000, 80], 0, 10, 8, 256, 64), ([200], [200], 50, 9, 3, 256, 16),
+    ([100, 17, 1], [90, 400, 333], 0, 5, 6, 128, 16), ([80], [2000], 300, 40, 1, 64, 64), ([256], [256], 1, 3, 8, 64, 16)])
+def test_attention_prompt_tiles(T, dtype, queries, lens, window, H, G, D, bs):
+    """Enough heads and requests that every type walks its keys in tiles of rows."""
+    _attend(T, np.random.default_rng(13), lens, queries, H, G, D, bs, dtype, window)
+
+
 @pytest.mark.parametrize("n", [1, 90])
 def test_attention_without_cu_and_strided(T, n):
     """Rows from a fused projection, a strided output, a wider table, and no bounds."""
@@ -369,6 +379,21 @@ def test_delta(T, dtype, Hk, Hv, Dk, Dv, lens):
     _near(after, rs, 1e-5)
     T.gated_delta(q, k, v, g, beta, S, cu_seqlens=_dev(cu, torch.int32), max_len=max(lens))        # in place
     assert torch.equal(S, after)
+    assert T.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("Dk,Dv", [(128, 128), (64, 112)])
+def test_delta_many_sequences(T, dtype, Dk, Dv):
+    """So many sequences that each unit of columns is one warp's."""
+    rng = np.random.default_rng(Dv)
+    lens = [int(x) for x in rng.integers(17, 80, 24)] + [0, 1]
+    cu = np.concatenate([[0], np.cumsum(lens)]).tolist()
+    q, k, v, g, beta, S = _rule_inputs(rng, cu[-1], 4, 8, Dk, Dv, dtype, len(lens))
+    ro, rs = R.gated_delta(q, k, v, g, beta, S, cu)
+    o, s = T.gated_delta(q, k, v, g, beta, S, cu_seqlens=_dev(cu, torch.int32), max_len=max(lens))
+    _near(o, ro, TOL[dtype])
+    _near(s, rs, 1e-5)
     assert T.device_error() == 0
 
 

@@ -49,6 +49,8 @@ int device() {
     }
     return dev;
 }
+}  // namespace
+// The current device's multiprocessors, 0 without a device (used by tsb_delta.cu too).
 int sm_count() {
     static std::atomic<int> known[kMaxDev];
     const int dev = device();
@@ -63,6 +65,7 @@ int sm_count() {
     }
     return n;
 }
+namespace {
 // A kernel's dynamic shared memory above 48 KB, granted once a device: `most` is the largest asked for so far.
 template <class K>
 bool allow_smem(K* kernel, std::atomic<int> (&most)[kMaxDev], int bytes) {
@@ -133,7 +136,7 @@ __device__ __forceinline__ int last_le(const int* a, int n, int64_t v) {
 // which block a token's position lands in follows from the prefix sums alone, so no CTA reads what another writes.
 // The stack of free blocks is free_list[0 .. n_free) with the blocks given back on top of it; the k-th block taken is
 // the k-th from the top.  What bounds it is the launch and the dependent loads (lengths, then list or table): at 8
-// requests nothing else is left, at 1000 requests and 33,000 tokens the slots' 8 bytes a token are 0.3 MB.
+// requests nothing else is left (5.2 us), at 1000 requests and 33,000 tokens the slots' 8 bytes a token are 0.3 MB (8.7 us).
 __global__ void __launch_bounds__(kTabThreads) k_block_tables(const TabParams p) {
     extern __shared__ int sh[];
     const int R = p.n_req;
@@ -313,11 +316,12 @@ __device__ __forceinline__ uint4 rescale_codes(uint4 w, float ratio) {
     return w;
 }
 
-// Warp (keys or values, head, token), for decode steps, where nearly every token is a run of its own.  A run is the tokens of one call that follow one another within one
-// cache block; its first token is the leader, and its warp takes the run: the largest magnitude over
-// it, the block's new scale max(old, largest / 127) (old: none when the run starts the block), the block's earlier codes
+// Warp (keys or values, head, token), for decode steps, where nearly every token is a run of its own.  A run is the tokens
+// of one call that follow one another within one cache block; its first token is the leader, and its warp takes the run:
+// the largest magnitude over it, the block's new scale max(old, largest / 127) (old: none when the run starts the block), the block's earlier codes
 // brought to it when it grew, and the run's codes.  One warp owns the (block, head), so no value is written twice and
-// nothing is atomic.  Divisions are IEEE: the same codes on any device.  Bound by the chain of loads: slots, rows, scale.
+// nothing is atomic.  Divisions are IEEE: the same codes on any device.  Bound by the chain of loads: slots, rows, scale
+// (48 tokens of 2 heads of 256: 3.2 us).
 __global__ void __launch_bounds__(128) k_kv8_append(const AppendParams p) {
     const int lane = threadIdx.x & 31;
     const int bs = p.c.bs, D = p.c.D, DV = D / 8, dvs = D == 64 ? 3 : D == 128 ? 4 : 5;
@@ -370,6 +374,7 @@ __global__ void __launch_bounds__(128) k_kv8_append(const AppendParams p) {
 
 // The same for prompts: CTA (chunk of block_size tokens, head, keys or values), the run's values in registers between the
 // two passes (up to 64 a thread; a warp's two passes over 16 KB went to memory twice: 82 us for 16,024 tokens of 8 heads).
+// Now 64 us for those in fp32, 164 MB: the codes' arithmetic and the memory about equally.
 __global__ void __launch_bounds__(128) k_kv8_append_runs(const AppendParams p) {
     __shared__ float peaks[4];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -451,7 +456,8 @@ __global__ void __launch_bounds__(128) k_kv8_append_runs(const AppendParams p) {
 }
 
 // CTA (share of the tokens, head, keys or values): four codes a thread and step, so that a warp's stores of 16 (8) bytes a
-// lane are consecutive, eight steps in flight.  A slot outside the cache reads as zeros.
+// lane are consecutive, eight steps in flight.  A slot outside the cache reads as zeros.  Bound by the bytes: 16,024 tokens of
+// 8 heads of 128 to fp32 (164 MB) take 45 us.
 constexpr int kReadSteps = 8;
 __global__ void __launch_bounds__(256) k_kv8_read(const Cache c, const int64_t* __restrict__ slots, int64_t n_tok,
                                                   void* k, void* v, int type) {
@@ -964,6 +970,9 @@ constexpr int kSplitCtas = NB == 1 ? (D == 256 ? 3 : D == 128 ? 4 : 5) : (D == 2
 // equal ranges, one per CTA; a range's warps take its steps in turn and join their rows through shared memory at the
 // end of each segment.  A segment inside one range is finished there; one cut by a range's end leaves its rows, maxima
 // and sums for k_attn_join.  So a lone request of 131,072 tokens and 64 requests of uneven lengths fill the GPU alike.
+// Bound by memory with one query a request (32 requests of 8192 tokens, heads of 128: 5.7 TB/s; 2 of 131,072, heads of 256,
+// fp32: 58 us, 4.6 TB/s), by the issue of the score planes' products with more (64 of up to 8192 with up to 3: 139 us,
+// 3.9 TB/s).
 template <int D, int SP, int NB>
 __global__ void __launch_bounds__(kAttnWarps * 32, kSplitCtas<D, NB>) k_attn_split(const __grid_constant__ AttnParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
@@ -1218,7 +1227,7 @@ __global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ AttnP
 
 // Many rows of fp32 queries: one warp per tile of 32 rows (head_dim 256: 16), every step of the tile by the same warp, which turns a
 // step's codes into operands once for all of them; the four warps of a CTA take neighbouring tiles of a head, so they share
-// the codes through the caches.
+// the codes through the caches.  Bound by the products, three planes a score: 843 queries of 8 heads over 2000 keys 209 us.
 template <int D>
 constexpr int kTileGroups = D == 256 ? 2 : 4;
 template <int D>

@@ -28,6 +28,7 @@ namespace tsb {
 
 void set_last_error(const char* msg);   // tsb_moe.cu: the text tsb_last_error returns
 unsigned* device_error_word();          // tsb_moe.cu: the current device's error word
+int sm_count();                         // tsb_cache.cu: the current device's multiprocessors
 
 namespace {
 
@@ -99,7 +100,8 @@ __device__ __forceinline__ float4 ld_state(const float* p) {     // volatile: is
 // CTA (32 value columns, value head, sequence): the state's slice in registers, thread (row group of 32, 4 columns):
 // dim_k / 32 rows of four columns.  One reduction over dim_k a token: S^T k and S^T q of the decayed state together,
 // o = scale (S^T q + (q . k) u), so the second product needs no second pass.  Single tokens are bound by the state's
-// bytes, read and written once.
+// bytes, read and written once: 128 of them with 32 heads of 128 x 128 (540 MB) take 119 us, 4.5 TB/s; 5, 6 and 8 CTAs a SM
+// measured 119, 129 and 160.
 template <int DK>
 __global__ void __launch_bounds__(256, 4) k_delta_step(const DeltaParams p) {
     constexpr int RPT = DK / 32;
@@ -363,7 +365,7 @@ __device__ __forceinline__ void merge_blocks(float* X, float* tmp, int tid) {
 // workspace; K K^T and Q K^T on the tensor cores (warp w: rows 16 w); then for each value head of the key head the
 // decays, A, P and M.  (1 + A)^-1 in fp32 from its 8 x 8 diagonal blocks (forward substitution, a thread a column) by
 // three joins of neighbouring blocks: exact arithmetic on the triangle, where powers of A would cancel, with every
-// thread at work (one thread a column over all 64 rows is 2000 dependent steps: 240 us for 8192 tokens, 32 heads).
+// thread at work (one thread a column over all 64 rows is 2000 dependent steps: 240 us for 8192 tokens, 32 heads; now 148).
 template <int E, int DK>
 __global__ void __launch_bounds__(128, E == E_F32 ? 2 : 4) k_delta_prepare(const DeltaParams p) {
     using T = Tiles<E, DK>;
@@ -652,7 +654,8 @@ struct RowScale {
 // Z and O, which no later chunk waits for, from the same exchanges, and bring V.  What bounds it: a sequence's chunks
 // follow one another, and a unit's 400 products of 16 x 8 x 16 a chunk (bf16, dim_k 128) at 8 cycles each.  One sequence
 // of 32 heads has 256 units, so W 2 puts them on 128 SMs with every scheduler at work; with more sequences W 1 does the
-// same work without exchanges.
+// same work without exchanges.  8192 tokens of 32 heads, bf16: 329 us, a chunk in 4670 cycles, of which the products before the
+// next chunk take 2140 and the exchanges 1590.
 template <int E, int DK, int W>
 __global__ void __launch_bounds__(256) k_delta_scan(const DeltaParams p) {
     using T = Tiles<E, DK>;
@@ -1195,8 +1198,13 @@ int launch_chunks(const DeltaParams& p, cudaStream_t st) {
         return dcuda("gated_delta: shared memory");
     k_delta_prepare<E, DK><<<dim3((unsigned) p.max_chunks, p.hk), 128, sm, st>>>(p);
     if (int rc = dcuda("gated_delta: chunks")) return rc;
-    // W 2 until there is work for every SM without it: 8 sequences of 1 to 1024 tokens, 32 heads: 177 us a pass against 208
-    return (int64_t) p.n_seq * p.hv >= 512 ? launch_scan<E, DK, 1>(p, st) : launch_scan<E, DK, 2>(p, st);
+    // W 1 does less in all and W 2 a chunk sooner, so W 1 where the chunks of all sequences outweigh the longest one's, and where its
+    // eight units a CTA have 16 columns each.  Measured with 32 heads of 128 (us a pass, W 1 against W 2): one sequence of 8192
+    // tokens 1324 against 477, 8 ragged ones up to 1024 208 against 174 (fp32); 4 of 1000 245 against 257 (fp32 268 against 334), 16
+    // of 256 259 against 276, 64 of 64 281 against 425; 16 of 256 with 6 heads 73 against 78; with heads of 64 143 against 128.
+    const int64_t longest = (p.max_len + kChunk - 1) / kChunk;
+    const bool many = p.dv > 64 && (int64_t) p.max_chunks * p.hv * 5 >= longest * sm_count() * 3;
+    return many ? launch_scan<E, DK, 1>(p, st) : launch_scan<E, DK, 2>(p, st);
 }
 template <int DK>
 int launch_type(const DeltaParams& p, cudaStream_t st) {
