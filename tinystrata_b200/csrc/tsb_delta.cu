@@ -100,14 +100,16 @@ __device__ __forceinline__ float4 ld_state(const float* p) {     // volatile: is
 // CTA (32 value columns, value head, sequence): the state's slice in registers, thread (row group of 32, 4 columns):
 // dim_k / 32 rows of four columns.  One reduction over dim_k a token: S^T k and S^T q of the decayed state together,
 // o = scale (S^T q + (q . k) u), so the second product needs no second pass.  Single tokens are bound by the state's
-// bytes, read and written once: 128 of them with 32 heads of 128 x 128 (540 MB) take 119 us, 4.5 TB/s; 5, 6 and 8 CTAs a SM
-// measured 119, 129 and 160.
+// bytes, read and written once: 128 of them with 32 heads of 128 x 128 (540 MB) take 103 us, 5.2 TB/s (119 while every thread
+// summed the warps' parts for its columns; one warp does it now); 5 and 6 CTAs a SM measured 105 and 111.
 template <int DK>
 __global__ void __launch_bounds__(256, 4) k_delta_step(const DeltaParams p) {
     constexpr int RPT = DK / 32;
     __shared__ float qk[2][DK];
     __shared__ float red[8][2][32];
     __shared__ float dots[8][3];
+    __shared__ __align__(16) float us[32];
+    __shared__ float fade;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int c4 = (tid & 7) * 4, rg = tid >> 3;
     const int col = blockIdx.x * 32 + c4, h = blockIdx.y, b = blockIdx.z;
@@ -130,12 +132,14 @@ __global__ void __launch_bounds__(256, 4) k_delta_step(const DeltaParams p) {
             qk[0][tid] = qv, qk[1][tid] = kv;
             dkk = kv * kv, dqq = qv * qv, dqk = qv * kv;
         }
-        float vv[4] = {0, 0, 0, 0};
-        if (in) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) vv[j] = load_elem(p.v, tok * p.v_tok + (int64_t) h * p.v_head + col + j, p.type);
+        // the last warp's lanes have a column each: its value, and below its u and its output
+        const int mine = blockIdx.x * 32 + lane;
+        const bool finish = warp == 7, col_in = mine < p.dv;
+        float v = 0.0f, g = 0.0f, beta = 0.0f;
+        if (finish) {
+            if (col_in) v = load_elem(p.v, tok * p.v_tok + (int64_t) h * p.v_head + mine, p.type);
+            g = p.g[tok * p.gb_tok + h], beta = p.beta[tok * p.gb_tok + h];
         }
-        const float decay = expf(p.g[tok * p.gb_tok + h]), beta = p.beta[tok * p.gb_tok + h];
         dkk = warp_sum(dkk), dqq = warp_sum(dqq), dqk = warp_sum(dqk);
         if (lane == 0) dots[warp][0] = dkk, dots[warp][1] = dqq, dots[warp][2] = dqk;
         __syncthreads();
@@ -161,29 +165,26 @@ __global__ void __launch_bounds__(256, 4) k_delta_step(const DeltaParams p) {
             for (int j = 0; j < 4; ++j) red[warp][0][c4 + j] = sk[j], red[warp][1][c4 + j] = sq[j];
         }
         __syncthreads();
-        float kk = 0.0f, qq = 0.0f, qdk = 0.0f;
+        if (finish) {
+            float kk = 0.0f, qq = 0.0f, qdk = 0.0f, a = 0.0f, c = 0.0f;
 #pragma unroll
-        for (int w = 0; w < DK / 32; ++w) kk += dots[w][0], qq += dots[w][1], qdk += dots[w][2];
-        const float rk = p.norm ? rsqrtf(kk + p.eps) : 1.0f, rq = p.norm ? rsqrtf(qq + p.eps) : 1.0f;
-        float u[4];
+            for (int w = 0; w < DK / 32; ++w) kk += dots[w][0], qq += dots[w][1], qdk += dots[w][2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float a = 0.0f, c = 0.0f;
-#pragma unroll
-            for (int w = 0; w < 8; ++w) a += red[w][0][c4 + j], c += red[w][1][c4 + j];
-            u[j] = beta * (vv[j] - decay * rk * a);
-            vv[j] = p.scale * rq * (decay * c + qdk * rk * u[j]);     // o
-            u[j] *= rk;
+            for (int w = 0; w < 8; ++w) a += red[w][0][lane], c += red[w][1][lane];
+            const float rk = p.norm ? rsqrtf(kk + p.eps) : 1.0f, rq = p.norm ? rsqrtf(qq + p.eps) : 1.0f, decay = expf(g);
+            const float u = beta * (v - decay * rk * a);
+            us[lane] = u * rk;
+            if (lane == 0) fade = decay;
+            if (col_in) store_elem(p.o, tok * p.o_tok + (int64_t) h * p.o_head + mine, p.type, p.scale * rq * (decay * c + qdk * rk * u));
         }
-        if (rg == 0 && in) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) store_elem(p.o, tok * p.o_tok + (int64_t) h * p.o_head + col + j, p.type, vv[j]);
-        }
+        __syncthreads();
+        const float4 u = *(const float4*) (us + c4);
+        const float decay = fade;
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
             const float kv = qk[1][i * 32 + rg];
-            S[i].x = fmaf(kv, u[0], S[i].x * decay), S[i].y = fmaf(kv, u[1], S[i].y * decay);
-            S[i].z = fmaf(kv, u[2], S[i].z * decay), S[i].w = fmaf(kv, u[3], S[i].w * decay);
+            S[i].x = fmaf(kv, u.x, S[i].x * decay), S[i].y = fmaf(kv, u.y, S[i].y * decay);
+            S[i].z = fmaf(kv, u.z, S[i].z * decay), S[i].w = fmaf(kv, u.w, S[i].w * decay);
         }
         if (t + 1 < s.n) __syncthreads();
     }
