@@ -100,13 +100,13 @@ __device__ __forceinline__ float4 ld_state(const float* p) {     // volatile: is
 // CTA (32 value columns, value head, sequence): the state's slice in registers, thread (row group of 32, 4 columns):
 // dim_k / 32 rows of four columns.  One reduction over dim_k a token: S^T k and S^T q of the decayed state together,
 // o = scale (S^T q + (q . k) u), so the second product needs no second pass.  Single tokens are bound by the state's
-// bytes, read and written once: 128 of them with 32 heads of 128 x 128 (540 MB) take 103 us, 5.2 TB/s (119 while every thread
-// summed the warps' parts for its columns; one warp does it now); 5 and 6 CTAs a SM measured 105 and 111.
+// bytes, read and written once: 128 of them with 32 heads of 128 x 128 (540 MB) take 100 us, 5.4 TB/s (119 while every thread
+// summed the warps' parts for its columns, which one warp does now); 5 and 6 CTAs a SM measured 105 and 111 against 103.
 template <int DK>
 __global__ void __launch_bounds__(256, 4) k_delta_step(const DeltaParams p) {
     constexpr int RPT = DK / 32;
     __shared__ float qk[2][DK];
-    __shared__ float red[8][2][32];
+    __shared__ __align__(16) float red[8][2][32];
     __shared__ float dots[8][3];
     __shared__ __align__(16) float us[32];
     __shared__ float fade;
@@ -152,18 +152,15 @@ __global__ void __launch_bounds__(256, 4) k_delta_step(const DeltaParams p) {
             sq[0] = fmaf(S[i].x, qv, sq[0]), sq[1] = fmaf(S[i].y, qv, sq[1]);
             sq[2] = fmaf(S[i].z, qv, sq[2]), sq[3] = fmaf(S[i].w, qv, sq[3]);
         }
+        // over the row groups of a warp: a lane keeps half of what it has at each of the two steps
+        const bool hi = lane & 8, odd = lane & 16;
+        float k4[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 4; ++j) k4[j] = (hi ? sq[j] : sk[j]) + __shfl_xor_sync(0xffffffffu, hi ? sk[j] : sq[j], 8);
+        float k2[2];
 #pragma unroll
-            for (int o = 8; o < 32; o <<= 1) {
-                sk[j] += __shfl_xor_sync(0xffffffffu, sk[j], o);
-                sq[j] += __shfl_xor_sync(0xffffffffu, sq[j], o);
-            }
-        }
-        if (lane < 8) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) red[warp][0][c4 + j] = sk[j], red[warp][1][c4 + j] = sq[j];
-        }
+        for (int j = 0; j < 2; ++j) k2[j] = (odd ? k4[2 + j] : k4[j]) + __shfl_xor_sync(0xffffffffu, odd ? k4[j] : k4[2 + j], 16);
+        *(float2*) &red[warp][hi][c4 + (odd ? 2 : 0)] = make_float2(k2[0], k2[1]);
         __syncthreads();
         if (finish) {
             float kk = 0.0f, qq = 0.0f, qdk = 0.0f, a = 0.0f, c = 0.0f;
