@@ -398,7 +398,8 @@ typedef struct tsb_kv8_attn {
     int32_t window;         /* a query sees the last `window` keys up to its own; 0: all of them */
     float scale;            /* of the scores */
     int64_t n_tok;          /* rows of q and out */
-    int64_t q_tok, q_head, o_tok, o_head, table_stride;
+    int64_t q_tok, q_head, o_tok, o_head;
+    int64_t table_stride;   /* between requests' rows, which are only read and may overlap (0: all requests share one) */
 } tsb_kv8_attn;
 uint64_t tsb_kv8_attention_workspace_bytes(const tsb_kv8* cache, const tsb_kv8_attn* d);
 /* Causal attention of each request's last queries over its cached keys (the queries' own among them): request r's rows

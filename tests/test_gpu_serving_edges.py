@@ -1,0 +1,46 @@
+"""The serving-step operators at the edges of what they accept: shared and overlapping rows, windows and lengths near the
+ends of 32 bits, values that are not finite, defaults, and arguments that the caller could get wrong unnoticed."""
+import numpy as np
+import pytest
+import torch
+
+from . import serving_ref as R
+from .test_gpu_serving import BF16, F16, F32, T, _attend, _cache, _dev, _hold, _keys_v, _near, _rule_inputs, _tables  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ table rows
+@pytest.mark.parametrize("n,dtype", [(1, BF16), (1, F32), (40, BF16), (500, BF16), (500, F32)])
+def test_attention_shared_table_rows(T, n, dtype):
+    """Requests that share a row of the table, all of one (stride 0) or with rows that overlap (a stride below the
+    width), give the outputs of the same rows laid out apart."""
+    rng = np.random.default_rng(21)
+    H, G, D, bs, L = 4, 4, 64, 16, 700
+    NB = 64
+    c = _cache(T, rng, NB, H, D, bs)
+    ids = _dev(rng.permutation(NB), torch.int32)
+    lens = _dev([L, L - 3, n], torch.int32)
+    q = torch.randn((3 * n, H * G, D), device="cuda").to(dtype)
+    for table in (ids[None, :44].expand(3, 44), ids.as_strided((3, 44), (5, 1))):
+        apart = table.contiguous()
+        assert table.stride(0) < 44 == apart.stride(0)
+        got = T.kv8_attention(c, q, table, lens, max_q=n)
+        assert torch.equal(got, T.kv8_attention(c, q, apart, lens, max_q=n))
+        ref, mag = R.attention(c.k, c.v, c.k_scale, c.v_scale, q, apart, lens.tolist(), [0, n, 2 * n, 3 * n], D ** -0.5, 0)
+        _hold(got, ref, mag, dtype, _keys_v(c, [L]))
+    assert T.device_error() == 0
+
+
+def test_block_tables_refuses_rows_that_share_memory(T):
+    one = torch.full((1, 4), -1, dtype=torch.int32, device="cuda")
+    room = torch.full((16,), -1, dtype=torch.int32, device="cuda")
+    kw = dict(free=_dev([0, 1, 2, 3], torch.int32), n_free=_dev([4], torch.int32), block_size=16, cap_tokens=3)
+    two = dict(lens=_dev([0, 0], torch.int32), n_new=_dev([1, 2], torch.int32), **kw)
+    for table in (one.expand(2, 4), room.as_strided((2, 4), (3, 1))):
+        with pytest.raises(T.TsbError, match="block_tables: table"):
+            T.block_tables(table=table, **two)
+    assert (one == -1).all() and (room == -1).all()
+    # a single row has no stride to speak of
+    p = T.block_tables(lens=_dev([0], torch.int32), n_new=_dev([3], torch.int32), table=room.as_strided((1, 4), (1, 1)), **kw)
+    assert p.slots.tolist() == [48, 49, 50] and room[:2].tolist() == [3, -1]

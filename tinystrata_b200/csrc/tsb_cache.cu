@@ -1465,7 +1465,7 @@ int tsb_kv8_attention(const tsb_kv8* cache, const tsb_kv8_attn* d, const void* q
     if (!q || !out || !lens || (!table && d->table_width)) return cfail(TSB_ERR_ARG, "kv8_attention: null pointer");
     if (!cu_q && d->n_tok < (int64_t) d->n_req * d->max_q)
         return cfail(TSB_ERR_ARG, "kv8_attention: without cu_q every request has max_q queries");
-    if (d->table_stride < d->table_width) return cfail(TSB_ERR_ARG, "kv8_attention: table_stride");
+    if (d->table_stride < 0) return cfail(TSB_ERR_ARG, "kv8_attention: table_stride");
     const int es = elem_bytes(d->elem_type);
     if ((uintptr_t) q % es || (uintptr_t) out % es) return cfail(TSB_ERR_ALIGN, "kv8_attention: element alignment");
     if (a.ws && (!workspace || ws_bytes < a.ws))

@@ -143,13 +143,15 @@ PyObject* block_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (done.defined()) flat(done, at::kByte, R, dev, "block_tables: done");
         const int64_t width = table.size(1), blocks = stack.size(0);
         if (table.size(0) < R || (width > 1 && table.stride(1) != 1)) bad(table, "block_tables: table", "a contiguous row for every request");
+        // the call writes every request's row: rows that share memory would be one another's
+        if (R > 1 && table.stride(0) < width) bad(table, "block_tables: table", "rows that do not overlap");
         need(cap >= 0, "block_tables: cap_tokens");
         need(R <= INT32_MAX && width <= INT32_MAX && blocks <= INT32_MAX, "block_tables: sizes");
         const c10::cuda::CUDAGuard guard(dev);
         at::Tensor after = at::empty({R}, lens.options()), cu = at::empty({R + 1}, lens.options()), left = at::empty({1}, lens.options()),
                    slots = at::empty({cap}, lens.options().dtype(at::kLong));
         status(tsb_block_tables((const int32_t*) ptr(lens), (const int32_t*) ptr(add), (const uint8_t*) ptr(done), (int) R,
-                                (int32_t*) ptr(table), std::max(table.stride(0), width), (int) width, (int32_t*) ptr(stack), (int) blocks,
+                                (int32_t*) ptr(table), R > 1 ? table.stride(0) : width, (int) width, (int32_t*) ptr(stack), (int) blocks,
                                 (const int32_t*) ptr(n_free), bs, (int32_t*) ptr(after), (int32_t*) ptr(cu), (int64_t*) ptr(slots), cap,
                                 (int32_t*) ptr(left), stream_of(dev)),
                "block_tables");
@@ -258,7 +260,7 @@ PyObject* kv8_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         d.max_q = int32(a[5], "kv8_attention: max_q"), d.window = int32(a[6], "kv8_attention: window");
         d.scale = a[7] == Py_None ? (float) (1.0 / std::sqrt((double) p.c.head_dim)) : (float) number(a[7]);
         d.n_tok = T, d.q_tok = q.stride(0), d.q_head = q.stride(1), d.o_tok = out.stride(0), d.o_head = out.stride(1);
-        d.table_stride = std::max(table.stride(0), width);
+        d.table_stride = R > 1 ? table.stride(0) : width;   // requests may share a row (an expanded table)
         const uint64_t size = tsb_kv8_attention_workspace_bytes(&p.c, &d);
         const at::Tensor ws = bytes(size, p.dev);
         status(tsb_kv8_attention(&p.c, &d, ptr(q), (const int32_t*) ptr(table), (const int32_t*) ptr(lens), (const int32_t*) ptr(cu),

@@ -57,8 +57,8 @@ def block_tables(lens, n_new, table, free, n_free, block_size: int, cap_tokens: 
     """One step of the cache's block allocator (tsb_block_tables): blocks for the step's new tokens off the stack ``free``
     (its first n_free[0] entries), blocks of the requests with ``done`` back onto it, and every new token's slot.
 
-    lens, n_new int32 [R], table int32 [R, W], free int32 [blocks], n_free int32 [1], done uint8 [R] or None.  ``table``
-    and ``free`` are updated in place."""
+    lens, n_new int32 [R], table int32 [R, W] (rows that do not overlap), free int32 [blocks], n_free int32 [1], done
+    uint8 [R] or None.  ``table`` and ``free`` are updated in place."""
     if stream is not None:
         with _on(stream):
             return block_tables(lens, n_new, table, free, n_free, block_size, cap_tokens, done)
@@ -111,7 +111,7 @@ def kv8_attention(cache: KV8Cache, q, table, lens, cu_q=None, max_q: int = 1, wi
     """Causal attention of each request's last queries over its cached keys and values (tsb_kv8_attention).
 
     q [T, q_heads, head_dim]; table int32 [R, W] and lens int32 [R] as ``block_tables`` leaves them (the queries' own keys
-    appended); cu_q int32 [R + 1] bounds of the requests' rows in q (None: max_q rows each); max_q at least the most rows
+    appended; requests may share rows of the table, as samples of one prompt do: ``table.expand``); cu_q int32 [R + 1] bounds of the requests' rows in q (None: max_q rows each); max_q at least the most rows
     of a request; window 0 or the number of last keys a query sees; scale default head_dim ** -0.5.  Returns out, of q's
     shape and type."""
     if stream is not None:
