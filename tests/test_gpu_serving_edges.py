@@ -44,3 +44,18 @@ def test_block_tables_refuses_rows_that_share_memory(T):
     # a single row has no stride to speak of
     p = T.block_tables(lens=_dev([0], torch.int32), n_new=_dev([3], torch.int32), table=room.as_strided((1, 4), (1, 1)), **kw)
     assert p.slots.tolist() == [48, 49, 50] and room[:2].tolist() == [3, -1]
+
+
+# ------------------------------------------------------------------------------------------------ windows
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 2, 1 << 30, 700])
+@pytest.mark.parametrize("queries,lens,H,G,D", [
+    ([4, 1, 3], [1, 700, 0], 2, 4, 128),                # few rows: split over CTAs
+    ([300, 300, 40], [1, 400, 0], 8, 4, 64)])           # tiles of rows
+def test_attention_windows_as_long_as_all_keys(T, dtype, window, queries, lens, H, G, D):
+    """A window that no request fills hides nothing, whatever its size, also where a request has more queries than keys
+    (its first rows have positions below zero)."""
+    _, _, _, wide = _attend(T, np.random.default_rng(22), lens, queries, H, G, D, 16, dtype, window)
+    _, _, _, all_of_them = _attend(T, np.random.default_rng(22), lens, queries, H, G, D, 16, dtype, 0)
+    assert torch.equal(wide, all_of_them)
+    assert T.device_error() == 0

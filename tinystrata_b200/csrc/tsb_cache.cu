@@ -539,6 +539,9 @@ __device__ __forceinline__ Req attn_req(const AttnParams& p, int r) {
     }
     return q;
 }
+// The first key of row i's window (below zero when it holds all of them).  A row without keys counts as position -1: the
+// difference stays in 32 bits for every window.
+__device__ __forceinline__ int window_first(const AttnParams& p, const Req& q, int i) { return max(q.len - q.n + i + 1, 0) - p.window; }
 // The steps [first, first + n) that the rows of tile rt (of TR rows) see.
 template <int TR>
 __device__ __forceinline__ void tile_steps(const AttnParams& p, const Req& q, int rt, int& first, int& n) {
@@ -546,7 +549,7 @@ __device__ __forceinline__ void tile_steps(const AttnParams& p, const Req& q, in
     first = n = 0;
     if (r0 >= rows) return;
     const int i0 = r0 / p.G, i1 = (min(r0 + TR, rows) - 1) / p.G;
-    const int hi = q.len - q.n + i1 + 1, lo = p.window > 0 ? max(0, q.len - q.n + i0 - p.window + 1) : 0;
+    const int hi = q.len - q.n + i1 + 1, lo = p.window > 0 ? max(0, window_first(p, q, i0)) : 0;
     if (hi <= 0) return;
     first = lo / kStep;
     n = (hi + kStep - 1) / kStep - first;
@@ -785,7 +788,7 @@ struct Walk {
                 rf[u][i] = rowf[u * 8 + 2 * qd + i];
             }
         const int pmin = q.len - q.n + (rt * TR) / p.G;
-        const int lmax = p.window > 0 ? q.len - q.n + (min(rt * TR + TR, rows) - 1) / p.G - p.window + 1 : INT_MIN;
+        const int lmax = p.window > 0 ? window_first(p, q, (min(rt * TR + TR, rows) - 1) / p.G) : INT_MIN;
         float ref = 0.0f, per_ref = 0.0f;                // SP 1: a power of two above the value scales so far, its inverse
         int stage = 0;
         for (; s < n; s += stride) {

@@ -158,9 +158,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_attn_prompt(const __grid_
         const int wq = warp & 3, half = warp >> 2;
         const uint32_t mine = tmem + ((uint32_t) (wq * 32) << 16);
         const int i = wq * 32 + lane, row = rt * 128 + i;
-        const int pos = q.len - q.n + min(row, rows - 1) / p.G;
+        const int pos = max(q.len - q.n + min(row, rows - 1) / p.G, -1);   // -1: no keys
         const int pmin = q.len - q.n + (rt * 128) / p.G;
-        const int lmax = p.window > 0 ? q.len - q.n + (min(rt * 128 + 128, rows) - 1) / p.G - p.window + 1 : INT_MIN;
+        const int lmax = p.window > 0 ? window_first(p, q, (min(rt * 128 + 128, rows) - 1) / p.G) : INT_MIN;
         const int win = p.window > 0 ? p.window : INT_MAX;
         const float rf = rowf[i];
         float m = -INFINITY, l = 0.0f, ref = 0.0f, per_ref = 0.0f;
