@@ -1315,8 +1315,9 @@ int attn_plan(const tsb_kv8* c, const tsb_kv8_attn* d, AttnPlan& a) {
     if (d->n_req > kMaxReq) return cfail(TSB_ERR_UNSUPPORTED, "kv8_attention: at most %d requests", kMaxReq);
     if (d->q_heads < 1 || d->q_heads % c->n_kv_heads)
         return cfail(TSB_ERR_ARG, "kv8_attention: q_heads %d not a multiple of the cache's %d heads", d->q_heads, c->n_kv_heads);
-    if ((int64_t) d->table_width * c->block_size > 0x7fffffffll - 64 || c->n_kv_heads > 65535)
-        return cfail(TSB_ERR_UNSUPPORTED, "kv8_attention: at most 2^31 tokens a request and 65535 heads");
+    // (k_attn_prompt looks up the blocks of up to three tiles of 128 tokens past a request's last in 32 bits)
+    if ((int64_t) d->table_width * c->block_size > 0x7fffffffll - 1024 || c->n_kv_heads > 65535)
+        return cfail(TSB_ERR_UNSUPPORTED, "kv8_attention: at most 2^31 - 1025 tokens a request and 65535 heads");
     a.G = d->q_heads / c->n_kv_heads;
     const int64_t rows = (int64_t) d->max_q * a.G;
     if (rows > (1 << 28)) return cfail(TSB_ERR_UNSUPPORTED, "kv8_attention: too many query rows");
