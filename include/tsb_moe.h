@@ -371,7 +371,7 @@ typedef struct tsb_kv8 {
  * Blocks given back go on top of it, blocks needed come from its top in request order; a request is served when its
  * blocks and all earlier requests' are there and its row is wide enough, else it keeps its length and blocks.
  * Writes lens_out, cu_new [n_req + 1] (prefix sums of n_new, refused requests' tokens included: they are in the caller's
- * packed rows), slots [cap_tokens] (block * block_size + offset of the step's tokens in packed order; -1 for a refused
+ * packed rows; held at 2^31 - 1 where they pass it), slots [cap_tokens] (block * block_size + offset of the step's tokens in packed order; -1 for a refused
  * request's and past the last), *n_free_out, the new entries of table, and free_list above the old top.  lens_out and
  * n_free_out must not be lens and n_free.  At most 8192 requests. */
 int tsb_block_tables(const int32_t* lens, const int32_t* n_new, const uint8_t* done, int n_req, int32_t* table,

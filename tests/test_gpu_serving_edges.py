@@ -59,3 +59,27 @@ def test_attention_windows_as_long_as_all_keys(T, dtype, window, queries, lens, 
     _, _, _, all_of_them = _attend(T, np.random.default_rng(22), lens, queries, H, G, D, 16, dtype, 0)
     assert torch.equal(wide, all_of_them)
     assert T.device_error() == 0
+
+
+# ------------------------------------------------------------------------------------------------ block tables
+def test_block_tables_requests_that_ask_for_too_much(T):
+    """Sums of the asked tokens and blocks beyond 32 bits: the requests that ask for them are refused, the others served,
+    and no token of the packed rows takes another request's slot."""
+    top = 2 ** 31 - 1
+    for new, cu, lens in (([top, top, 5], [0, top, top, top], [20, 3, 12]), ([5, top, top], [0, 5, top, top], [25, 3, 7]),
+                          ([0, top, 5], [0, 0, top, top], [20, 3, 12]), ([top, 0, 0], [0, top, top, top], [20, 3, 7])):
+        table = _dev([[4, 0, -1], [5, -1, -1], [1, -1, -1]], torch.int32)
+        p = T.block_tables(_dev([20, 3, 7], torch.int32), _dev(new, torch.int32), table, _dev([2, 3, 9, 9], torch.int32),
+                           _dev([2], torch.int32), 16, 8)
+        assert p.cu.tolist() == cu and p.lens.tolist() == lens and p.n_free.tolist() == [2]
+        first = [4, 5, 6, 7, 8] if new[0] == 5 else []
+        assert p.slots.tolist() == first + [-1] * (8 - len(first))
+        assert table.tolist() == [[4, 0, -1], [5, -1, -1], [1, -1, -1]]
+    # far more requests than blocks: the first in order are served
+    n = 4096
+    rows = torch.full((n, 4), -1, dtype=torch.int32, device="cuda")
+    p = T.block_tables(torch.zeros(n, dtype=torch.int32, device="cuda"), torch.full((n,), 64, dtype=torch.int32, device="cuda"), rows,
+                       torch.arange(10, dtype=torch.int32, device="cuda"), _dev([10], torch.int32), 16, n * 64)
+    assert p.lens.tolist() == [64, 64] + [0] * (n - 2) and p.n_free.tolist() == [2]
+    assert rows[:2].tolist() == [[9, 8, 7, 6], [5, 4, 3, 2]] and (rows[2:] == -1).all()
+    assert (p.slots[128:] == -1).all() and p.slots[0].item() == 9 * 16

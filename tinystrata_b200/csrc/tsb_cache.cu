@@ -143,24 +143,26 @@ __global__ void __launch_bounds__(kTabThreads) k_block_tables(const TabParams p)
     int* cu = sh;                     // R + 1
     int* take = sh + (R + 1);         // R + 1
     int* give = sh + 2 * (R + 1);     // R + 1
-    __shared__ int wsum[3][kTabThreads / 32];
+    __shared__ int64_t wsum[3][kTabThreads / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (R + kTabThreads - 1) / kTabThreads;
     const int r0 = min(tid * per, R), r1 = min(r0 + per, R);
     const int held = min(max(*p.n_free, 0), p.cap_free);
-    int s[3] = {0, 0, 0};
+    // Sums in 64 bits, stored as at most 2^31 - 1: refused requests count with whatever they ask for, and each prefix has to
+    // stay at or above the one before, since the searches below index with their differences.
+    int64_t s[3] = {0, 0, 0};
     for (int r = r0; r < r1; ++r) {
         const TabReq q = tab_req(p, r);
         cu[r] = q.add, take[r] = q.takes, give[r] = q.gives;      // this thread's own, sums below
         s[0] += q.add, s[1] += q.takes, s[2] += q.gives;
     }
-    int x[3];
+    int64_t x[3];
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
-        int v = s[i];
+        int64_t v = s[i];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, v, o);
+            const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
             if (lane >= o) v += u;
         }
         if (lane == 31) wsum[i][warp] = v;
@@ -171,12 +173,13 @@ __global__ void __launch_bounds__(kTabThreads) k_block_tables(const TabParams p)
     for (int i = 0; i < 3; ++i) {
         for (int w = 0; w < warp; ++w) x[i] += wsum[i][w];
     }
+    auto stored = [](int64_t v) { return (int) min(v, (int64_t) INT32_MAX); };
     for (int r = r0; r < r1; ++r) {
         const int add = cu[r], takes = take[r], gives = give[r];
-        cu[r] = x[0], take[r] = x[1], give[r] = x[2];
+        cu[r] = stored(x[0]), take[r] = stored(x[1]), give[r] = stored(x[2]);
         x[0] += add, x[1] += takes, x[2] += gives;
     }
-    if (tid == kTabThreads - 1) cu[R] = x[0], take[R] = x[1], give[R] = x[2];
+    if (tid == kTabThreads - 1) cu[R] = stored(x[0]), take[R] = stored(x[1]), give[R] = stored(x[2]);
     __syncthreads();
 
     const int given = min(give[R], p.cap_free - held);
