@@ -83,3 +83,28 @@ def test_block_tables_requests_that_ask_for_too_much(T):
     assert p.lens.tolist() == [64, 64] + [0] * (n - 2) and p.n_free.tolist() == [2]
     assert rows[:2].tolist() == [[9, 8, 7, 6], [5, 4, 3, 2]] and (rows[2:] == -1).all()
     assert (p.slots[128:] == -1).all() and p.slots[0].item() == 9 * 16
+
+
+# ------------------------------------------------------------------------------------------------ outputs
+def test_outputs_that_share_memory_are_refused(T):
+    """Rows of out that are one another's, and states after that lie across the states before."""
+    c = T.KV8Cache(4, 2, 64)
+    q, table, lens = torch.zeros((2, 8, 64), device="cuda"), torch.zeros((2, 2), dtype=torch.int32, device="cuda"), _dev([1, 1], torch.int32)
+    room = torch.full((2000,), 7.0, device="cuda")
+    for out in (room[:512].view(1, 8, 64).expand(2, 8, 64), room[:128].view(2, 1, 64).expand(2, 8, 64),
+                room.as_strided((2, 8, 64), (500, 64, 1)), room.as_strided((2, 8, 64), (512, 60, 1))):
+        with pytest.raises(T.TsbError, match="kv8_attention: out.*share memory"):
+            T.kv8_attention(c, q, table, lens, out=out)
+    x, v = torch.zeros((3, 1, 64), device="cuda"), torch.zeros((3, 2, 32), device="cuda")
+    g, S = torch.zeros((3, 2), device="cuda"), torch.full((4, 2, 64, 32), 7.0, device="cuda")
+    ok = dict(q=x, k=x, v=v, g=g, beta=g, state=S[:3], max_len=1)
+    with pytest.raises(T.TsbError, match="gated_delta: out.*share memory"):
+        T.gated_delta(**ok, out=room[:64].view(1, 2, 32).expand(3, 2, 32))
+    with pytest.raises(T.TsbError, match="gated_delta: state_out"):
+        T.gated_delta(**ok, state_out=S[1:])
+    assert (room == 7).all() and (S == 7).all()
+    # strided outputs of every order are taken
+    for out in (room[:1024].view(8, 2, 64).transpose(0, 1), room.as_strided((2, 8, 64), (900, 65, 1)), room[:1024].view(2, 8, 64)):
+        out.fill_(7)
+        T.kv8_attention(c, q, table, lens, out=out)
+        assert (out == 0).all()

@@ -89,6 +89,19 @@ void rows(const at::Tensor& t, int64_t n, int64_t heads, int64_t dim, at::Scalar
     if (t.size(0) != n || t.size(1) != heads || t.size(2) != dim || (dim > 1 && t.stride(2) != 1))
         bad(t, what, "[" + std::to_string(n) + ", " + std::to_string(heads) + ", " + std::to_string(dim) + "] with a contiguous innermost dimension");
 }
+// An output whose elements are all its own: strides, smallest first, step past what the smaller dimensions span.
+void own_memory(const at::Tensor& t, const char* what) {
+    int order[8];
+    const int n = (int) t.dim();
+    for (int i = 0; i < n; ++i) order[i] = i;
+    std::sort(order, order + n, [&](int a, int b) { return t.stride(a) < t.stride(b); });
+    int64_t span = 1;
+    for (int i = 0; i < n; ++i) {
+        if (t.size(order[i]) <= 1) continue;
+        if (t.stride(order[i]) < span) bad(t, what, "elements that do not share memory");
+        span += (t.size(order[i]) - 1) * t.stride(order[i]);
+    }
+}
 c10::Device cuda_of(const at::Tensor& t, const char* what) {
     if (!t.is_cuda()) bad(t, what, "a tensor on a CUDA device");
     return t.device();
@@ -254,7 +267,7 @@ PyObject* kv8_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (cu.defined()) flat(cu, at::kInt, R + 1, p.dev, "kv8_attention: cu_q");
         need(R <= INT32_MAX && heads <= INT32_MAX && width <= INT32_MAX, "kv8_attention: sizes");
         const c10::cuda::CUDAGuard guard(p.dev);
-        if (out.defined()) rows(out, T, heads, p.c.head_dim, q.scalar_type(), p.dev, "kv8_attention: out");
+        if (out.defined()) rows(out, T, heads, p.c.head_dim, q.scalar_type(), p.dev, "kv8_attention: out"), own_memory(out, "kv8_attention: out");
         else out = at::empty({T, heads, p.c.head_dim}, q.options());
         d.n_req = (int32_t) R, d.q_heads = (int32_t) heads, d.table_width = (int32_t) width;
         d.max_q = int32(a[5], "kv8_attention: max_q"), d.window = int32(a[6], "kv8_attention: window");
@@ -302,6 +315,9 @@ PyObject* gated_delta(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (state.size(1) != hv || state.size(2) != dk || state.size(3) != dv || !state.is_contiguous())
             bad(state, "gated_delta: state", "contiguous [n_states, v_heads, dim_k, dim_v]");
         if (after.sizes() != state.sizes() || !after.is_contiguous()) bad(after, "gated_delta: state_out", "contiguous, as state,");
+        const char *s0 = (const char*) ptr(state), *s1 = (const char*) ptr(after);
+        if (s0 != s1 && s0 < s1 + after.nbytes() && s1 < s0 + state.nbytes())
+            bad(after, "gated_delta: state_out", "state itself or memory of its own");
         const int64_t max_len = a[7] == Py_None ? T : integer(a[7]), slots = state.size(0);
         int64_t B;
         if (cu.defined()) {
@@ -317,7 +333,7 @@ PyObject* gated_delta(PyObject*, PyObject* const* a, Py_ssize_t n) {
         else need(slots >= B, "gated_delta: a state for every sequence");
         need(max_len >= 0 && max_len <= INT32_MAX && B <= INT32_MAX && slots <= INT32_MAX && hv <= INT32_MAX && dv <= INT32_MAX, "gated_delta: sizes");
         const c10::cuda::CUDAGuard guard(dev);
-        if (out.defined()) rows(out, T, hv, dv, type, dev, "gated_delta: out");
+        if (out.defined()) rows(out, T, hv, dv, type, dev, "gated_delta: out"), own_memory(out, "gated_delta: out");
         else out = at::empty({T, hv, dv}, q.options());
         d.n_seq = (int32_t) B, d.max_len = (int32_t) max_len, d.k_heads = (int32_t) hk, d.v_heads = (int32_t) hv;
         d.dim_k = (int32_t) dk, d.dim_v = (int32_t) dv, d.n_states = (int32_t) slots;

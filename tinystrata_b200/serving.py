@@ -113,7 +113,7 @@ def kv8_attention(cache: KV8Cache, q, table, lens, cu_q=None, max_q: int = 1, wi
     q [T, q_heads, head_dim]; table int32 [R, W] and lens int32 [R] as ``block_tables`` leaves them (the queries' own keys
     appended; requests may share rows of the table, as samples of one prompt do: ``table.expand``); cu_q int32 [R + 1] bounds of the requests' rows in q (None: max_q rows each); max_q at least the most rows
     of a request; window 0 or the number of last keys a query sees; scale default head_dim ** -0.5.  Returns out, of q's
-    shape and type."""
+    shape and type (elements that share no memory)."""
     if stream is not None:
         with _on(stream):
             return kv8_attention(cache, q, table, lens, cu_q, max_q, window, scale, out)
@@ -128,7 +128,8 @@ def gated_delta(q, k, v, g, beta, state, cu_seqlens=None, max_len: int | None = 
     q, k [T, k_heads, dim_k], v [T, v_heads, dim_v] of one type; g (log decays) and beta fp32 [T, v_heads]; state fp32
     [n_states, v_heads, dim_k, dim_v].  cu_seqlens int32 [B + 1] bounds the sequences (None: T / max_len sequences of
     max_len tokens; max_len default T, else at least the longest one).  state_idx int32 [B] names the sequences' states
-    (None: in order; negative: from zeros, not kept).  The states after the step go to state_out (default: in place).
+    (None: in order; negative: from zeros, not kept).  The states after the step go to state_out (default: in place; else
+    memory of its own), where states that no sequence names stay as they are.  out shares no memory with q and k.
     scale default dim_k ** -0.5; qk_norm divides q and k by sqrt(sum of squares + eps) first.  Returns (out, states)."""
     if stream is not None:
         with _on(stream):
