@@ -108,3 +108,22 @@ def test_outputs_that_share_memory_are_refused(T):
         out.fill_(7)
         T.kv8_attention(c, q, table, lens, out=out)
         assert (out == 0).all()
+
+
+# ------------------------------------------------------------------------------------------------ gated delta rule
+# k heads, v heads, dim_k, dim_v, sequences: two warps a unit (64 and 128 wide), and one (many sequences)
+RULE_FORMS = [(1, 2, 64, 64, 1), (2, 4, 128, 128, 1), (4, 8, 128, 128, 30)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [5, 17, 64, 65, 200])
+@pytest.mark.parametrize("Hk,Hv,Dk,Dv,B", RULE_FORMS)
+def test_delta_norm_without_eps(T, dtype, n, Hk, Hv, Dk, Dv, B):
+    """qk_norm with eps 0: the tokens that fill up a chunk are no division by zero."""
+    rng = np.random.default_rng(31)
+    q, k, v, g, beta, S = _rule_inputs(rng, B * n, Hk, Hv, Dk, Dv, dtype, B)
+    q, k = (q.float() * 3).to(dtype), (k.float() * 0.1).to(dtype)
+    ro, rs = R.gated_delta(q, k, v, g, beta, S, [b * n for b in range(B + 1)], qk_norm=True, eps=0.0)
+    o, s = T.gated_delta(q, k, v, g, beta, S, max_len=n, qk_norm=True, eps=0.0)
+    _near(o, ro, {F32: 1e-5, BF16: 5e-3}[dtype])
+    _near(s, rs, 1e-5)

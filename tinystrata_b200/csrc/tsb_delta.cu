@@ -422,7 +422,8 @@ __global__ void __launch_bounds__(128, E == E_F32 ? 2 : 4) k_delta_prepare(const
                 }
                 float up, inv;
                 pow2_scale(peak, up, inv);
-                if (piece == 0) (w ? rq : rk)[row] = p.norm ? rsqrtf(sq + p.eps) * inv : inv;
+                // (rows past the last token are zeros and have no length to divide by: with eps 0 that would be infinite)
+                if (piece == 0) (w ? rq : rk)[row] = p.norm && row < live ? rsqrtf(sq + p.eps) * inv : inv;
                 uint32_t hi[4], lo[4];
 #pragma unroll
                 for (int m = 0; m < 4; ++m) split_f16(x[i][2 * m] * up, x[i][2 * m + 1] * up, hi[m], lo[m]);
