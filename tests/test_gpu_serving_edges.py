@@ -127,3 +127,20 @@ def test_delta_norm_without_eps(T, dtype, n, Hk, Hv, Dk, Dv, B):
     o, s = T.gated_delta(q, k, v, g, beta, S, max_len=n, qk_norm=True, eps=0.0)
     _near(o, ro, {F32: 1e-5, BF16: 5e-3}[dtype])
     _near(s, rs, 1e-5)
+
+
+@pytest.mark.parametrize("n", [9, 16, 17, 64, 200])
+@pytest.mark.parametrize("Hk,Hv,Dk,Dv,B", RULE_FORMS)
+def test_delta_gate_that_is_not_a_number(T, n, Hk, Hv, Dk, Dv, B):
+    """A NaN decay makes its head's state NaN from its token on, in the recurrence and in chunks alike; -inf empties it."""
+    rng = np.random.default_rng(32)
+    q, k, v, g, beta, S = _rule_inputs(rng, B * n, Hk, Hv, Dk, Dv, F32, B)
+    at = (B - 1) * n + n // 2                               # in the last sequence
+    g[at, Hv - 1], g[at, 0] = float("nan"), float("-inf")
+    ro, rs = R.gated_delta(q, k, v, g, beta, S, [b * n for b in range(B + 1)])
+    o, s = T.gated_delta(q, k, v, g, beta, S, max_len=n)
+    assert torch.isnan(o[at:, Hv - 1]).all() and torch.isnan(s[B - 1, Hv - 1]).all()
+    o, s, ro, rs = o[:, :Hv - 1], s[:, :Hv - 1], ro[:, :Hv - 1], rs[:, :Hv - 1]
+    _near(o, ro, 1e-5)
+    _near(s, rs, 1e-5)
+    assert T.device_error() == 0

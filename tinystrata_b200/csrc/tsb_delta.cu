@@ -481,8 +481,8 @@ __global__ void __launch_bounds__(128, E == E_F32 ? 2 : 4) k_delta_prepare(const
     for (int i = 0; i < rep; ++i) {
         const int h = hk * rep + i;
         __syncthreads();                                  // the tiles, or the previous head's planes, are out
-        // e^-200 is 0 in fp32; a sum of -inf would make differences undefined
-        if (tid < 64) gc[tt] = (double) fmaxf(gnext, -200.0f);
+        // e^-200 is 0 in fp32; a sum of -inf would make differences undefined.  NaN stays NaN.
+        if (tid < 64) gc[tt] = (double) (gnext < -200.0f ? -200.0f : gnext);
         else beta[tt] = gnext;
         if (i + 1 < rep && tt < live) gnext = gsrc[i + 1];
         __syncthreads();
