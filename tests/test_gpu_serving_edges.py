@@ -144,3 +144,31 @@ def test_delta_gate_that_is_not_a_number(T, n, Hk, Hv, Dk, Dv, B):
     _near(o, ro, 1e-5)
     _near(s, rs, 1e-5)
     assert T.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [16, 40, 64, 200])
+@pytest.mark.parametrize("Hk,Hv,Dk,Dv,B", RULE_FORMS)
+@pytest.mark.parametrize("what", ["q", "k", "v", "g", "beta", "state"])
+def test_delta_values_that_are_not_finite(T, what, dtype, n, Hk, Hv, Dk, Dv, B):
+    """A token's NaN or infinity reaches what the recurrence says and nothing else: outputs of earlier tokens, other heads,
+    other columns (a value's) and other sequences stay as they are."""
+    rng = np.random.default_rng(33)
+    cu = [b * n for b in range(B + 1)]
+    clean = _rule_inputs(rng, B * n, Hk, Hv, Dk, Dv, dtype, B)
+    for at, bad in ((0, "nan"), (n // 2 + 3, "inf"), (n - 1, "nan"), (n // 3, "inf" if what in ("g", "beta") else "-inf")):
+        q, k, v, g, beta, S = (x.clone() for x in clean)
+        t = (B - 1) * n + at
+        if what == "state":
+            S[B - 1, Hv - 1, Dk // 2, 5] = float(bad)
+        elif what in ("g", "beta"):
+            (g if what == "g" else beta)[t, Hv - 1] = float(bad)
+        else:
+            {"q": q, "k": k, "v": v}[what][t, -1, 9] = float(bad)
+        ro, rs = R.gated_delta(q, k, v, g, beta, S, cu)
+        o, s = T.gated_delta(q, k, v, g, beta, S, max_len=n)
+        for got, ref, tol in ((o, ro, {F32: 1e-5, BF16: 5e-3}[dtype]), (s, rs, 1e-5)):
+            good = torch.isfinite(ref)
+            assert torch.equal(torch.isfinite(got), good), (at, bad)
+            _near(got.where(good, 0), ref.where(good, 0), tol)
+    assert T.device_error() == 0

@@ -16,6 +16,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <climits>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -48,6 +49,9 @@ int dcuda(const char* what) {
 }
 
 constexpr int kChunk = 64;
+constexpr float kFinite = 3.4028235e38f;         // the largest finite value
+constexpr uint32_t kFiniteBits = 0x7f7fffffu;
+#define kNaN __uint_as_float(0x7fffffffu)
 constexpr unsigned kSiteDelta = 0xD0000001u;   // the error word when the scan's wait for a chunk's tiles gave up
 
 struct DeltaParams {
@@ -233,6 +237,12 @@ __device__ __forceinline__ float pow2f(float x) {
 __device__ __forceinline__ float max4(float a, float b, float c, float d) {
     return fmaxf(fmaxf(fabsf(a), fabsf(b)), fmaxf(fabsf(c), fabsf(d)));
 }
+// The largest of a, |x| and |y|, NaN if any is.
+__device__ __forceinline__ float max_nan(float a, float x, float y) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(fabsf(x)), "f"(fabsf(y)));
+    return r;
+}
 __device__ __forceinline__ float quad_max(float v) {
     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
     return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
@@ -376,6 +386,8 @@ __global__ void __launch_bounds__(128, E == E_F32 ? 2 : 4) k_delta_prepare(const
     float* tmp = A + kChunk * LA;                        // [32][36]
     __shared__ __align__(16) float rk[kChunk], rq[kChunk], beta[kChunk];
     __shared__ __align__(16) double gc[kChunk];
+    __shared__ bool k_lost[kChunk];
+    __shared__ uint32_t lost[4];
     __shared__ int sh[8];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int hk = blockIdx.y, rep = p.hv / p.hk;
@@ -409,21 +421,31 @@ __global__ void __launch_bounds__(128, E == E_F32 ? 2 : 4) k_delta_prepare(const
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
                 const int e = e0 + 128 * i, row = e / TPR, piece = e % TPR;
-                float sq = 0.0f, peak = 0.0f;
+                float sq = 0.0f, len = 1.0f;
+                uint32_t peak = 0;                        // by bits: above every finite value for NaN as for infinity
 #pragma unroll
-                for (int m = 0; m < 8; ++m) peak = fmaxf(peak, fabsf(x[i][m]));
+                for (int m = 0; m < 8; ++m) peak = max(peak, __float_as_uint(x[i][m]) & 0x7fffffffu);
 #pragma unroll
-                for (int o = TPR / 2; o > 0; o >>= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+                for (int o = TPR / 2; o > 0; o >>= 1) peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, o));
                 if (p.norm) {
 #pragma unroll
                     for (int m = 0; m < 8; ++m) sq = fmaf(x[i][m], x[i][m], sq);
 #pragma unroll
                     for (int o = TPR / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+                    if (row < live) len = rsqrtf(sq + p.eps);         // (the zeros past the last token have no length)
+                }
+                if (w == 0) {                             // a key that is not finite: zeros, and the head's states are lost below
+                    const bool gone = peak > kFiniteBits || !(len <= kFinite);
+                    if (gone) {
+                        peak = 0, len = 1.0f;
+#pragma unroll
+                        for (int m = 0; m < 8; ++m) x[i][m] = 0.0f;
+                    }
+                    if (piece == 0) k_lost[row] = gone;
                 }
                 float up, inv;
-                pow2_scale(peak, up, inv);
-                // (rows past the last token are zeros and have no length to divide by: with eps 0 that would be infinite)
-                if (piece == 0) (w ? rq : rk)[row] = p.norm && row < live ? rsqrtf(sq + p.eps) * inv : inv;
+                pow2_scale(__uint_as_float(peak), up, inv);
+                if (piece == 0) (w ? rq : rk)[row] = len * inv;
                 uint32_t hi[4], lo[4];
 #pragma unroll
                 for (int m = 0; m < 4; ++m) split_f16(x[i][2 * m] * up, x[i][2 * m + 1] * up, hi[m], lo[m]);
@@ -481,9 +503,15 @@ __global__ void __launch_bounds__(128, E == E_F32 ? 2 : 4) k_delta_prepare(const
     for (int i = 0; i < rep; ++i) {
         const int h = hk * rep + i;
         __syncthreads();                                  // the tiles, or the previous head's planes, are out
-        // e^-200 is 0 in fp32; a sum of -inf would make differences undefined.  NaN stays NaN.
-        if (tid < 64) gc[tt] = (double) (gnext < -200.0f ? -200.0f : gnext);
-        else beta[tt] = gnext;
+        // A token whose key, decay or beta is not finite (a decay of -inf is) leaves a state without a finite value, and outputs
+        // from itself on.  In the products it would reach the chunk's earlier tokens too, as 0 * NaN above the diagonals; so
+        // it takes part as zeros, and what it spoils is marked in the vectors.
+        const bool gone = tt < live && (tid < 64 ? k_lost[tt] || !(gnext <= kFinite) : !(fabsf(gnext) <= kFinite));
+        const unsigned any = __ballot_sync(0xffffffffu, gone);
+        if (lane == 0) lost[warp] = any;
+        // e^-200 is 0 in fp32; a sum of -inf would make differences undefined
+        if (tid < 64) gc[tt] = gone ? 0.0 : (double) fmaxf(gnext, -200.0f);
+        else beta[tt] = gone ? 0.0f : gnext;
         if (i + 1 < rep && tt < live) gnext = gsrc[i + 1];
         __syncthreads();
         if (warp == 0) {                                  // running sums, in units of log 2
@@ -499,15 +527,17 @@ __global__ void __launch_bounds__(128, E == E_F32 ? 2 : 4) k_delta_prepare(const
             }
             v[1] += __shfl_sync(0xffffffffu, v[0], 31);
             const double last = __shfl_sync(0xffffffffu, v[1], 31);
+            const unsigned l0 = lost[0] | lost[2], l1 = lost[1] | lost[3];
+            const int from = l0 ? __ffs(l0) - 1 : l1 ? __ffs(l1) + 31 : kChunk;        // the first lost token
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 const int t = w * 32 + lane;
                 gc[t] = v[w];
                 const float e = pow2f((float) v[w]);
                 vec[V_EK + t] = e * rk[t];
-                vec[V_EQ + t] = e * rq[t] * p.scale;
+                vec[V_EQ + t] = t < from ? e * rq[t] * p.scale : kNaN;
                 vec[V_ED + t] = pow2f((float) (last - v[w])) * rk[t];
-                vec[V_END + t] = pow2f((float) last);
+                vec[V_END + t] = from == kChunk ? pow2f((float) last) : kNaN;
             }
         }
         __syncthreads();
@@ -655,8 +685,13 @@ struct RowScale {
 // of 32 heads has 256 units, so W 2 puts them on 128 SMs with every scheduler at work; with more sequences W 1 does the
 // same work without exchanges.  8192 tokens of 32 heads, bf16: 329 us, a chunk in 4670 cycles, of which the products before the
 // next chunk take 2140 and the exchanges 1590.
+// W 2 at dim_k 128 fills a SM's shared memory with one CTA, and is told so: with the 128 registers that two would leave it
+// 8192 tokens take 496 us a pass, with 227 461.  The other forms are left to the compiler (W 1 told the same: 257 against
+// 240 for 16 sequences of 256).
+template <int DK, int W>
+constexpr int kScanCtas = W == 2 && DK == 128 ? 1 : 0;
 template <int E, int DK, int W>
-__global__ void __launch_bounds__(256) k_delta_scan(const DeltaParams p) {
+__global__ void __launch_bounds__(256, kScanCtas<DK, W>) k_delta_scan(const DeltaParams p) {
     using T = Tiles<E, DK>;
     constexpr int PL = T::PL;
     constexpr bool OS = T::PP == 2;
@@ -669,6 +704,7 @@ __global__ void __launch_bounds__(256) k_delta_scan(const DeltaParams p) {
     __shared__ uint64_t full[2], empty[2];
     __shared__ int sh[8];
     __shared__ float peaks[UN][4][W][16];
+    __shared__ int lost[UN][16];                       // a column's first token (of the sequence) whose X is not finite
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, qd = lane & 3;
     const bool writer = W == 2 && warp >= 4;           // W 2: warps 0-3 carry the states of two units, 4-7 write the outputs
     const int unit = (warp & (UN * W - 1)) / W, part = warp % W;
@@ -683,6 +719,7 @@ __global__ void __launch_bounds__(256) k_delta_scan(const DeltaParams p) {
     uint4* fs = (uint4*) (sm + 2 * T::kStage + unit * kFrag);   // S [DK / 16][2][32]; later U e^(gc_63 - gc) [4][2][32]
     uint4* fu = fs + 256;                                       // U [4][2][32]
     uint4* fx = fs + 512;                                       // X [4][2][32]
+    if (tid < UN * 16) (&lost[0][0])[tid] = INT_MAX;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 8);
         fence_mbar_init();
@@ -817,9 +854,34 @@ __global__ void __launch_bounds__(256) k_delta_scan(const DeltaParams p) {
             Z[n][0] *= eq.x * rs.i[0], Z[n][1] *= eq.y * rs.i[0], Z[n][2] *= eq.x * rs.i[1], Z[n][3] *= eq.y * rs.i[1];
         }
     };
+    // X^T of chunk c with zeros for what is not finite (a value, or the state): such a token spoils its column from itself
+    // on, but as 0 * NaN it would reach the tokens before it.  Also the rows' largest magnitudes.
+    auto clean = [&](int c, float (&X)[NP * 2][4], float& a, float& cc) {
+        a = cc = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NP * 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (!(fabsf(X[n][e]) <= kFinite)) {
+                    atomicMin(&lost[unit][g + (e >> 1) * 8], c * kChunk + tile_of(n >> 1) * 16 + (n & 1) * 8 + 2 * qd + (e & 1));
+                    X[n][e] = 0.0f;
+                }
+                if (e < 2) a = fmaxf(a, fabsf(X[n][e]));
+                else cc = fmaxf(cc, fabsf(X[n][e]));
+            }
+    };
     // O^T = Z^T + U^T P^T of chunk c, from U's left operands
-    auto outputs = [&](int c, uint32_t mr, const float* vec, const float (&Z)[NP * 2][4], const uint32_t (&xh)[4][4], const uint32_t (&xl)[4][4]) {
+    auto outputs = [&](int c, uint32_t mr, const float* vec, float (&Z)[NP * 2][4], const uint32_t (&xh)[4][4], const uint32_t (&xl)[4][4]) {
         const int live = in ? min(kChunk, s.n - c * kChunk) : 0;
+        const int from[2] = {lost[unit][g], lost[unit][g + 8]};
+        if (__any_sync(0xffffffffu, min(from[0], from[1]) < (c + 1) * kChunk)) {
+#pragma unroll
+            for (int n = 0; n < NP * 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c * kChunk + tile_of(n >> 1) * 16 + (n & 1) * 8 + 2 * qd + (e & 1) >= from[e >> 1]) Z[n][e] = kNaN;
+            __syncwarp();
+        }
         float O[NP * 2][4];
 #pragma unroll
         for (int n = 0; n < NP * 2; ++n)
@@ -1004,13 +1066,19 @@ __global__ void __launch_bounds__(256) k_delta_scan(const DeltaParams p) {
             else v = ((const float4*) fx)[(tile_of(n >> 1) * 2 + (n & 1)) * 32 + lane];
             Y[n][0] = fmaf(-ek.x * rs.i[0], Y[n][0], v.x), Y[n][1] = fmaf(-ek.y * rs.i[0], Y[n][1], v.y);
             Y[n][2] = fmaf(-ek.x * rs.i[1], Y[n][2], v.z), Y[n][3] = fmaf(-ek.y * rs.i[1], Y[n][3], v.w);
-            a = fmaxf(a, fmaxf(fabsf(Y[n][0]), fabsf(Y[n][1])));
-            cc = fmaxf(cc, fmaxf(fabsf(Y[n][2]), fabsf(Y[n][3])));
+            a = max_nan(a, Y[n][0], Y[n][1]);
+            cc = max_nan(cc, Y[n][2], Y[n][3]);
         }
+        bool cut = false;                           // X had to be cleaned
         if (W == 1 && c + 1 < chunks) load_values(c + 1);   // they arrive during the rest of this chunk
 
         uint32_t xh[4][4], xl[4][4];               // X's left operands, all token tiles; then U's
         if constexpr (W == 1) {
+            cut = __any_sync(0xffffffffu, !(a <= kFinite && cc <= kFinite));
+            if (cut) {
+                clean(c, Y, a, cc);
+                __syncwarp();
+            }
             tell_peak(a, cc, 1);
             rx.set(a, cc);
 #pragma unroll
@@ -1019,6 +1087,8 @@ __global__ void __launch_bounds__(256) k_delta_scan(const DeltaParams p) {
 #pragma unroll
             for (int n = 0; n < NP; ++n) put(fx, tile_of(n), Y[2 * n], Y[2 * n + 1], rx);
             if (pair_any(unit, !rx.holds(a, cc))) {
+                cut = true;
+                clean(c, Y, a, cc);
                 tell_peak(a, cc, 1);
                 pair_sync(unit);
                 join_peak(a, cc, 1);
@@ -1131,6 +1201,14 @@ __global__ void __launch_bounds__(256) k_delta_scan(const DeltaParams p) {
             for (int x = 0; x < 2 * NS; ++x)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) S[2 * n + x][e] = fmaf(acc[x][e], end_f[e >> 1], S[2 * n + x][e] * end);
+        }
+        if (cut) {                                  // columns that were lost up to here have no state
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                if (lost[unit][g + 8 * x] >= (c + 1) * kChunk) continue;
+#pragma unroll
+                for (int n = 0; n < NK; ++n) S[n][2 * x] = S[n][2 * x + 1] = kNaN;
+            }
         }
         if (W == 1) outputs(c, mr, vec, Z, xh, xl);
         release(c);
