@@ -431,7 +431,8 @@ uint64_t tsb_gated_delta_workspace_bytes(const tsb_delta_desc* d);
 /* n_seq sequences through the rule: rows cu_seqlens[b] .. cu_seqlens[b + 1] (null: max_len rows each) from state_in
  * [n_states][v_heads][dim_k][dim_v], the states after them to state_out (which may be state_in).  state_idx [n_seq]
  * (null: sequence b has state b) names each sequence's state, no two the same; a negative one starts from zeros and is
- * not kept.  Up to 16 tokens a sequence run token by token, longer ones in chunks of 64. */
+ * not kept, and so does one of n_states or more, which the device error word records; it records a sequence that is longer
+ * than max_len or reaches past n_tok too, whose further tokens are left out.  Up to 16 tokens a sequence run token by token, longer ones in chunks of 64. */
 int tsb_gated_delta(const tsb_delta_desc* d, const void* q, const void* k, const void* v, const float* g, const float* beta,
                     const float* state_in, float* state_out, const int32_t* state_idx, const int32_t* cu_seqlens, void* o,
                     void* workspace, uint64_t ws_bytes, void* stream);

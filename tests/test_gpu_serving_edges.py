@@ -172,3 +172,26 @@ def test_delta_values_that_are_not_finite(T, what, dtype, n, Hk, Hv, Dk, Dv, B):
             assert torch.equal(torch.isfinite(got), good), (at, bad)
             _near(got.where(good, 0), ref.where(good, 0), tol)
     assert T.device_error() == 0
+
+
+@pytest.mark.parametrize("n", [2, 70])
+def test_delta_says_what_it_leaves_out(T, n):
+    """A state that there is not, a sequence longer than max_len and one that reaches past the rows: left out, and recorded
+    in the device error word."""
+    rng = np.random.default_rng(34)
+    q, k, v, g, beta, S = _rule_inputs(rng, 2 * n, 2, 4, 128, 64, F32, 3)
+    kw = dict(q=q, k=k, v=v, g=g, beta=beta)
+    cu = [0, n, 2 * n]
+    assert T.device_error() == 0
+    for idx, error in (([2, 3], 0xD0000002), ([2, 2 ** 31 - 1], 0xD0000002), ([2, -1], 0), ([2, -7], 0)):
+        S2 = S.clone()
+        o, _ = T.gated_delta(**kw, state=S2, max_len=n, state_idx=_dev(idx, torch.int32))
+        assert T.device_error() == error
+        ro, rs = R.gated_delta(q, k, v, g, beta, S, cu, [2, -1])
+        _near(o, ro, 1e-5)
+        _near(S2, rs, 1e-5)
+        assert torch.equal(S2[:2], S[:2])
+    for bounds, longest, error in (([0, n, 2 * n], n - 1, 0xD0000003), ([0, n, 2 * n + 1], n + 1, 0xD0000003), ([0, n, 2 * n], n + 5, 0),
+                                   ([0, n, n], n, 0)):
+        T.gated_delta(**kw, state=S.clone(), cu_seqlens=_dev(bounds, torch.int32), max_len=longest)
+        assert T.device_error() == error

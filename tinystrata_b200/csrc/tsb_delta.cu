@@ -52,7 +52,9 @@ constexpr int kChunk = 64;
 constexpr float kFinite = 3.4028235e38f;         // the largest finite value
 constexpr uint32_t kFiniteBits = 0x7f7fffffu;
 #define kNaN __uint_as_float(0x7fffffffu)
-constexpr unsigned kSiteDelta = 0xD0000001u;   // the error word when the scan's wait for a chunk's tiles gave up
+constexpr unsigned kSiteDelta = 0xD0000001u;   // the error word when the scan's wait for a chunk's tiles gave up,
+constexpr unsigned kSiteState = 0xD0000002u;   // when state_idx names a state that there is not,
+constexpr unsigned kSiteLong = 0xD0000003u;    // and when a sequence is longer than max_len or reaches past n_tok
 
 struct DeltaParams {
     const void *q, *k, *v;
@@ -94,6 +96,11 @@ __device__ __forceinline__ int state_of(const DeltaParams& p, int b) {
     const int i = p.idx ? p.idx[b] : b;
     return i >= 0 && i < p.n_states ? i : -1;
 }
+// What the device's own counts ask beyond the caller's sizes is left out, and said in the error word.
+__device__ __forceinline__ void check_sequence(const DeltaParams& p, int b) {
+    if (p.idx && p.idx[b] >= p.n_states) report_error(p.err, kSiteState);
+    if (p.cu && (int64_t) p.cu[b + 1] > min((int64_t) max(p.cu[b], 0) + p.max_len, p.n_tok)) report_error(p.err, kSiteLong);
+}
 
 // ------------------------------------------------------------------------------------------------ recurrence
 __device__ __forceinline__ float4 ld_state(const float* p) {     // volatile: issued where it stands
@@ -126,6 +133,7 @@ __global__ void __launch_bounds__(256, 4) k_delta_step(const DeltaParams p) {
     for (int i = 0; i < RPT; ++i)
         S[i] = st >= 0 && in ? ld_state(p.s_in + base + (int64_t) (i * 32 + rg) * p.dv) : make_float4(0, 0, 0, 0);
     const Seq s = seq_of(p, b);      // after the state's loads are on their way: nothing before them waits for memory
+    if (blockIdx.x == 0 && h == 0 && tid == 0) check_sequence(p, b);
     if (s.n == 0 && p.s_in == p.s_out) return;
     for (int t = 0; t < s.n; ++t) {
         const int64_t tok = s.tok + t;
@@ -723,6 +731,7 @@ __global__ void __launch_bounds__(256, kScanCtas<DK, W>) k_delta_scan(const Delt
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 8);
         fence_mbar_init();
+        if (blockIdx.x == 0 && h == 0) check_sequence(p, b);
     }
     __syncthreads();
     const int64_t cb = T::chunk_bytes(p.hk, p.hv);
@@ -1328,6 +1337,7 @@ int tsb_gated_delta(const tsb_delta_desc* d, const void* q, const void* k, const
     p.scale = d->scale, p.eps = d->eps, p.norm = d->qk_norm != 0;
     p.wide = !((uintptr_t) q % 16 || (uintptr_t) k % 16 || (p.q_tok * es) % 16 || (p.q_head * es) % 16 || (p.k_tok * es) % 16 ||
                (p.k_head * es) % 16);
+    p.err = device_error_word();
     cudaStream_t st = (cudaStream_t) stream;
     if (d->max_len <= kStepTokens) {
         const dim3 grid((d->dim_v + 31) / 32, d->v_heads, d->n_seq);
@@ -1342,7 +1352,6 @@ int tsb_gated_delta(const tsb_delta_desc* d, const void* q, const void* k, const
     if (max_chunks(d) > 0x7fffffffll) return dfail(TSB_ERR_UNSUPPORTED, "gated_delta: too many tokens");
     p.ws = (uint8_t*) workspace;
     p.max_chunks = (int) max_chunks(d);
-    p.err = device_error_word();
     return d->dim_k == 64 ? launch_type<64>(p, st) : launch_type<128>(p, st);
 }
 
