@@ -110,6 +110,31 @@ def test_outputs_that_share_memory_are_refused(T):
         assert (out == 0).all()
 
 
+# ------------------------------------------------------------------------------------------------ rows of the requests
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("queries,lens,H,G", [([3, 1, 2], [90, 40, 2], 2, 4), ([300, 5, 140], [400, 5, 140], 8, 4)])
+def test_attention_every_row_by_default(T, dtype, queries, lens, H, G):
+    """Bounds without max_q leave no row out; with too small a max_q the request is cut, which the device error word says."""
+    rng = np.random.default_rng(23)
+    c, table, q, got = _attend(T, rng, lens, queries, H, G, 64, 16, dtype)
+    cu = _dev([0, *np.cumsum(queries).tolist()], torch.int32)
+    out = torch.full_like(q, 7.0)
+    T.kv8_attention(c, q, table, _dev(lens, torch.int32), cu_q=cu, out=out)
+    assert T.device_error() == 0
+    ref, mag = R.attention(c.k, c.v, c.k_scale, c.v_scale, q, table, lens, cu.tolist(), 64 ** -0.5, 0)
+    _hold(out, ref, mag, dtype, _keys_v(c, lens))
+    T.kv8_attention(c, q, table, _dev(lens, torch.int32), cu_q=cu, max_q=max(queries) - 1)
+    assert T.device_error() == 0xC0000002
+    T.kv8_attention(c, q[:-1], table, _dev(lens, torch.int32), cu_q=cu, max_q=max(queries))
+    assert T.device_error() == 0xC0000002
+    # rows of no request stay as they are
+    few = _dev([0, *np.cumsum(queries).tolist()[:-1], sum(queries[:-1])], torch.int32)
+    out.fill_(7)
+    T.kv8_attention(c, q, table, _dev(lens, torch.int32), cu_q=few, out=out)
+    assert (out[sum(queries[:-1]):] == 7).all() and torch.isfinite(out).all()
+    assert T.device_error() == 0
+
+
 # ------------------------------------------------------------------------------------------------ gated delta rule
 # k heads, v heads, dim_k, dim_v, sequences: two warps a unit (64 and 128 wide), and one (many sequences)
 RULE_FORMS = [(1, 2, 64, 64, 1), (2, 4, 128, 128, 1), (4, 8, 128, 128, 30)]

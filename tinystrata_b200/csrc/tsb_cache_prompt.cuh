@@ -107,6 +107,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_attn_prompt(const __grid_
     const int rt = gridDim.x - 1 - blockIdx.x, h = blockIdx.y, r = blockIdx.z;
     const Req q = attn_req(p, r);
     const int rows = q.n * p.G;
+    if (rt == 0 && h == 0 && tid == 0) check_request(p, r);
     if (rt * 128 >= rows) return;
     int first, steps;
     tile_steps<128>(p, q, rt, first, steps);

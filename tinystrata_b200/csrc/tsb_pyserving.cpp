@@ -246,7 +246,7 @@ PyObject* kv8_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// (cache, q, table, lens, cu_q, max_q, window, scale or None, out or None) -> out
+// (cache, q, table, lens, cu_q, max_q or None, window, scale or None, out or None) -> out
 PyObject* kv8_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         count(n, 9);
@@ -270,7 +270,9 @@ PyObject* kv8_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (out.defined()) rows(out, T, heads, p.c.head_dim, q.scalar_type(), p.dev, "kv8_attention: out"), own_memory(out, "kv8_attention: out");
         else out = at::empty({T, heads, p.c.head_dim}, q.options());
         d.n_req = (int32_t) R, d.q_heads = (int32_t) heads, d.table_width = (int32_t) width;
-        d.max_q = int32(a[5], "kv8_attention: max_q"), d.window = int32(a[6], "kv8_attention: window");
+        if (a[5] != Py_None) d.max_q = int32(a[5], "kv8_attention: max_q");
+        else d.max_q = cu.defined() ? (int32_t) std::min<int64_t>(T, INT32_MAX) : 1;
+        d.window = int32(a[6], "kv8_attention: window");
         d.scale = a[7] == Py_None ? (float) (1.0 / std::sqrt((double) p.c.head_dim)) : (float) number(a[7]);
         d.n_tok = T, d.q_tok = q.stride(0), d.q_head = q.stride(1), d.o_tok = out.stride(0), d.o_head = out.stride(1);
         d.table_stride = R > 1 ? table.stride(0) : width;   // requests may share a row (an expanded table)

@@ -106,14 +106,16 @@ def kv8_read(cache: KV8Cache, slots, dtype=torch.float32, stream=None):
     return (_native or _load()).kv8_read(cache._pools, slots, _ELEM[dtype])
 
 
-def kv8_attention(cache: KV8Cache, q, table, lens, cu_q=None, max_q: int = 1, window: int = 0, scale: float | None = None,
+def kv8_attention(cache: KV8Cache, q, table, lens, cu_q=None, max_q: int | None = None, window: int = 0, scale: float | None = None,
                   out=None, stream=None):
     """Causal attention of each request's last queries over its cached keys and values (tsb_kv8_attention).
 
     q [T, q_heads, head_dim]; table int32 [R, W] and lens int32 [R] as ``block_tables`` leaves them (the queries' own keys
-    appended; requests may share rows of the table, as samples of one prompt do: ``table.expand``); cu_q int32 [R + 1] bounds of the requests' rows in q (None: max_q rows each); max_q at least the most rows
-    of a request; window 0 or the number of last keys a query sees; scale default head_dim ** -0.5.  Returns out, of q's
-    shape and type (elements that share no memory)."""
+    appended; requests may share rows of the table, as samples of one prompt do: ``table.expand``); cu_q int32 [R + 1]
+    bounds of the requests' rows in q (None: max_q rows each); max_q at least the most rows of a request (default 1, with
+    cu_q all rows of q; a close bound is faster, and a request with more rows is cut and recorded in ``device_error()``);
+    window 0 or the number of last keys a query sees; scale default head_dim ** -0.5.  Returns out, of q's shape and type
+    (its elements share no memory); rows of no request stay as out had them (a new one: undefined)."""
     if stream is not None:
         with _on(stream):
             return kv8_attention(cache, q, table, lens, cu_q, max_q, window, scale, out)
