@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import tinystrata_b200 as T
+from tinystrata_b200 import serving
 
 from .test_serving_host import ALIGN, ARG, CUDA, UNSUP, WS, attend, built, cache, desc, rule, tables  # noqa: F401
 
@@ -19,3 +20,27 @@ def test_attention_lengths_near_the_end_of_32_bits(block):
         assert attend(c, table_width=width, table_stride=width) == UNSUP
         d = desc(table_width=width, table_stride=width)
         assert T.lib().tsb_kv8_attention_workspace_bytes(C.byref(c), C.byref(d)) == 0
+
+
+def test_cache_calls_see_the_tensors_it_has(monkeypatch):
+    """A pool that was assigned anew is the one the calls get, and sizes are the pools'."""
+    seen = []
+
+    class Native:
+        kv8_append = staticmethod(lambda pools, *a: seen.append(pools))
+        kv8_read = staticmethod(lambda pools, *a: seen.append(pools))
+        kv8_attention = staticmethod(lambda pools, *a: seen.append(pools))
+
+    monkeypatch.setattr(serving, "_native", Native)
+    c = T.KV8Cache(4, 2, 64, device="cpu")
+    x, i = torch.zeros((1, 2, 64)), torch.zeros(1, dtype=torch.int64)
+    c.k, c.v = (torch.zeros((6, 3, 32, 128), dtype=torch.int8) for _ in "kv")
+    c.k_scale, c.v_scale = (torch.zeros((6, 3)) for _ in "kv")
+    del seen[:]
+    T.kv8_append(c, x, x, i)
+    T.kv8_read(c, i)
+    T.kv8_attention(c, x, i, i)
+    assert len(seen) == 3
+    for pools in seen:
+        assert all(a is b for a, b in zip(pools, (c.k, c.v, c.k_scale, c.v_scale)))
+    assert (c.n_blocks, c.n_kv_heads, c.block_size, c.head_dim) == (6, 3, 32, 128)

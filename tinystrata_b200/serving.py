@@ -80,11 +80,16 @@ class KV8Cache:
             raise TsbError(f"KV8Cache: [n_blocks, n_kv_heads, block_size 16 | 32 | 64, head_dim 64 | 128 | 256] wanted, got "
                            f"{tuple(k.shape)}")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.n_blocks, self.n_kv_heads, self.block_size, self.head_dim = k.shape
-        self._pools = (k, v, k_scale, v_scale)
         kv8_append(self, k.new_empty((0, self.n_kv_heads, self.head_dim), dtype=torch.float32),
                    k.new_empty((0, self.n_kv_heads, self.head_dim), dtype=torch.float32),
                    k.new_empty(0, dtype=torch.int64))             # checks the four tensors
+
+    n_blocks = property(lambda self: self.k.shape[0])
+    n_kv_heads = property(lambda self: self.k.shape[1])
+    block_size = property(lambda self: self.k.shape[2])
+    head_dim = property(lambda self: self.k.shape[3])
+    # what the calls take: the tensors as they are now
+    _pools = property(lambda self: (self.k, self.v, self.k_scale, self.v_scale))
 
 
 def kv8_append(cache: KV8Cache, k, v, slots, stream=None) -> None:
