@@ -220,3 +220,32 @@ def test_delta_says_what_it_leaves_out(T, n):
                                    ([0, n, n], n, 0)):
         T.gated_delta(**kw, state=S.clone(), cu_seqlens=_dev(bounds, torch.int32), max_len=longest)
         assert T.device_error() == error
+
+
+# ------------------------------------------------------------------------------------------------ threads
+def test_calls_of_threads_with_sizes_of_their_own(T):
+    """Host threads whose calls ask for different amounts of shared memory (by their requests) at once, then the largest."""
+    import threading
+    rng = np.random.default_rng(24)
+    c = _cache(T, rng, 8, 1, 64, 16)
+    errors = []
+
+    def work(n):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    z = torch.zeros(n, dtype=torch.int32, device="cuda")
+                    T.block_tables(z, z, torch.zeros((n, 1), dtype=torch.int32, device="cuda"), z[:1], z[:1], 16, 0)
+                    m = min(n, 4096)
+                    T.kv8_attention(c, torch.zeros((m, 2, 64), device="cuda"), torch.zeros((m, 1), dtype=torch.int32, device="cuda"), z[:m])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                                # noqa: BLE001
+            errors.append((n, e))
+    threads = [threading.Thread(target=work, args=(n,)) for n in (8192, 4200, 6000, 5000, 4097, 7000, 8000, 3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    work(8192)
+    assert not errors and T.device_error() == 0

@@ -8,7 +8,7 @@ import torch
 import tinystrata_b200 as T
 from tinystrata_b200 import serving
 
-from .test_serving_host import ALIGN, ARG, CUDA, UNSUP, WS, attend, built, cache, desc, rule, tables  # noqa: F401
+from .test_serving_host import A, ALIGN, ARG, CUDA, UNSUP, WS, attend, built, cache, desc, rule, tables  # noqa: F401
 
 
 @pytest.mark.parametrize("block", [16, 32, 64])
@@ -44,3 +44,12 @@ def test_cache_calls_see_the_tensors_it_has(monkeypatch):
     for pools in seen:
         assert all(a is b for a, b in zip(pools, (c.k, c.v, c.k_scale, c.v_scale)))
     assert (c.n_blocks, c.n_kv_heads, c.block_size, c.head_dim) == (6, 3, 32, 128)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the pointers are not real")
+def test_no_device_is_an_error():
+    """A call that cannot reach a device says so, whatever its size."""
+    for n in (1, 4, 5000, 8192):
+        assert tables(n=n) == CUDA, n
+        assert "block_tables" in T.last_error()
+    assert attend() == CUDA and attend(n_req=4000, cu=A, n_tok=8000) == CUDA

@@ -66,16 +66,16 @@ int sm_count() {
     return n;
 }
 namespace {
-// A kernel's dynamic shared memory above 48 KB, granted once a device: `most` is the largest asked for so far.
+// The most dynamic shared memory that a kernel can ask for, granted once a device.  (Always the same size: the attribute is
+// set, not raised, so that two threads with sizes of their own could leave the smaller one.)
 template <class K>
-bool allow_smem(K* kernel, std::atomic<int> (&most)[kMaxDev], int bytes) {
-    if (bytes <= 48 * 1024) return true;
+int allow_smem(K* kernel, std::atomic<bool> (&granted)[kMaxDev], int most, const char* what) {
     const int dev = device();
-    if (dev < 0) return false;
-    if (most[dev].load(std::memory_order_relaxed) >= bytes) return true;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
-    most[dev].store(bytes, std::memory_order_relaxed);
-    return true;
+    if (dev < 0) return cfail(TSB_ERR_CUDA, "%s: no CUDA device", what);
+    if (granted[dev].load(std::memory_order_acquire)) return TSB_OK;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess) return ccuda(what);
+    granted[dev].store(true, std::memory_order_release);
+    return TSB_OK;
 }
 
 // ------------------------------------------------------------------------------------------------ block tables
@@ -1357,9 +1357,10 @@ int attn_plan(const tsb_kv8* c, const tsb_kv8_attn* d, AttnPlan& a) {
 
 template <int D, int SP, int NB>
 int launch_split(const AttnParams& p, const AttnPlan& a, int rows, cudaStream_t st) {
-    static std::atomic<int> most[kMaxDev];
-    const int sm = kAttnWarps * Ring<D>::kBytes + NB * (3 * (D / 32) * 256 + kAttnWarps * 64 + 32) + (p.n_req + 1) * 8;
-    if (!allow_smem(k_attn_split<D, SP, NB>, most, sm)) return ccuda("kv8_attention: shared memory");
+    static std::atomic<bool> granted[kMaxDev];
+    constexpr int fixed = kAttnWarps * Ring<D>::kBytes + NB * (3 * (D / 32) * 256 + kAttnWarps * 64 + 32);
+    const int sm = fixed + (p.n_req + 1) * 8;
+    if (int rc = allow_smem(k_attn_split<D, SP, NB>, granted, fixed + (kMaxReq + 1) * 8, "kv8_attention: shared memory")) return rc;
     k_attn_split<D, SP, NB><<<a.n_cta, kAttnWarps * 32, sm, st>>>(p);
     if (int rc = ccuda("kv8_attention")) return rc;
     // the join's CTAs come up while the split runs; each waits for it (griddepcontrol.wait) before it reads its results
@@ -1378,8 +1379,8 @@ int launch_split(const AttnParams& p, const AttnPlan& a, int rows, cudaStream_t 
 }
 template <int D, bool LO>
 int launch_prompt(const AttnParams& p, cudaStream_t st) {
-    static std::atomic<int> most[kMaxDev];
-    if (!allow_smem(k_attn_prompt<D, LO>, most, Prompt<D, LO>::kAsk)) return ccuda("kv8_attention: shared memory");
+    static std::atomic<bool> granted[kMaxDev];
+    if (int rc = allow_smem(k_attn_prompt<D, LO>, granted, Prompt<D, LO>::kAsk, "kv8_attention: shared memory")) return rc;
     k_attn_prompt<D, LO><<<dim3((unsigned) p.tiles, p.c.H, p.n_req), kPromptThreads, Prompt<D, LO>::kAsk, st>>>(p);
     return ccuda("kv8_attention");
 }
@@ -1388,9 +1389,9 @@ int launch_attn(const AttnParams& p, const AttnPlan& a, int rows, cudaStream_t s
     if (a.split) return a.groups == 1 ? launch_split<D, SP, 1>(p, a, rows, st) : launch_split<D, SP, 2>(p, a, rows, st);
     if (a.prompt) return launch_prompt<D, SP == 2>(p, st);
     if constexpr (SP == 2) {                 // fp32 queries (a 16-bit prompt went to launch_prompt)
-        static std::atomic<int> most[kMaxDev];
+        static std::atomic<bool> granted[kMaxDev];
         const int sm = kAttnWarps * (kTileGroups<D> * 3 * (D / 32) * 256 + 128 + Ring<D>::kBytes);
-        if (!allow_smem(k_attn_tiles<D>, most, sm)) return ccuda("kv8_attention: shared memory");
+        if (int rc = allow_smem(k_attn_tiles<D>, granted, sm, "kv8_attention: shared memory")) return rc;
         if (p.cu) k_attn_check<<<1, 256, 0, st>>>(p);
         k_attn_tiles<D><<<dim3((unsigned) ((p.tiles + kAttnWarps - 1) / kAttnWarps), p.c.H, p.n_req), kAttnWarps * 32, sm, st>>>(p);
     }
@@ -1426,8 +1427,8 @@ int tsb_block_tables(const int32_t* lens, const int32_t* n_new, const uint8_t* d
     const TabParams p{lens, n_new, done, n_req, table, table_stride, table_width, free_list, free_cap, n_free, block_size,
                       lens_out, cu_new, slots, cap_tokens, n_free_out};
     const int sm = 3 * (n_req + 1) * 4;
-    static std::atomic<int> most[kMaxDev];
-    if (!allow_smem(k_block_tables, most, sm)) return ccuda("block_tables: shared memory");
+    static std::atomic<bool> granted[kMaxDev];
+    if (int rc = allow_smem(k_block_tables, granted, 3 * (kTabMaxReq + 1) * 4, "block_tables: shared memory")) return rc;
     // a thread a token, and for blocks that may be given back
     const int64_t work = std::max<int64_t>({cap_tokens, n_req, (int64_t) n_req * table_width / 16});
     const int ctas = (int) std::min<int64_t>(std::max<int64_t>((work + kTabThreads - 1) / kTabThreads, 1), std::max(2 * sm_count(), 1));
