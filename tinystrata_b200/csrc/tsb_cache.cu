@@ -1161,6 +1161,11 @@ __global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ AttnP
     __shared__ float stat[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int seg_id = blockIdx.x;
+    if (seg_id == (int) gridDim.x - 1) {                     // past the segments: the requests' bounds
+        if (blockIdx.y == 0)
+            for (int i = threadIdx.x; i < p.n_req; i += 256) check_request(p, i);
+        return;
+    }
     const int rt = seg_id % p.tiles, h = seg_id / p.tiles % p.c.H, r = seg_id / p.tiles / p.c.H;
     const Req q = attn_req(p, r);
     int first, n;
@@ -1172,7 +1177,6 @@ __global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ AttnP
     tile_steps<TR>(p, q, rt, first, n);
     const int cost = step_cost<TR>(p, q, rt);
     const int items = min(max(q.n * p.G - rt * TR, 0), TR) * (D / 64);
-    if (rt == 0 && h == 0 && blockIdx.y == 0 && threadIdx.x == 0) check_request(p, r);
     asm volatile("griddepcontrol.wait;" ::: "memory");       // every CTA: the split is complete from here on
     if (items == 0) return;
     const int64_t total = p.pre[p.n_req], p0 = p.pre[r], p1 = p.pre[r + 1], per_cta = units_per_cta(total, p.n_cta);
@@ -1366,7 +1370,7 @@ int launch_split(const AttnParams& p, const AttnPlan& a, int rows, cudaStream_t 
     // the join's CTAs come up while the split runs; each waits for it (griddepcontrol.wait) before it reads its results
     cudaLaunchConfig_t cfg{};
     const int segs = p.n_req * p.c.H * p.tiles, items = std::min(rows, 8 * NB) * (D / 64);
-    cfg.gridDim = dim3((unsigned) segs, (unsigned) std::max(1, std::min(items, a.n_cta / segs)));
+    cfg.gridDim = dim3((unsigned) segs + 1, (unsigned) std::max(1, std::min(items, a.n_cta / segs)));
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute at{};
@@ -1491,7 +1495,7 @@ int tsb_kv8_attention(const tsb_kv8* cache, const tsb_kv8_attn* d, const void* q
     if (a.ws && (!workspace || ws_bytes < a.ws))
         return cfail(TSB_ERR_WORKSPACE, "kv8_attention: workspace of %llu bytes needed", (unsigned long long) a.ws);
     if (a.ws && (uintptr_t) workspace % 16) return cfail(TSB_ERR_ALIGN, "kv8_attention: 16-byte aligned workspace");
-    if ((int64_t) d->n_req * cache->n_kv_heads * a.tiles > 0x7fffffffll || d->n_req > 65535)
+    if ((int64_t) d->n_req * cache->n_kv_heads * a.tiles > 0x7ffffffell || d->n_req > 65535)
         return cfail(TSB_ERR_UNSUPPORTED, "kv8_attention: too many requests");
     AttnParams p{};
     p.c = cache_of(cache);
