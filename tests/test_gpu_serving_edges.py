@@ -249,3 +249,53 @@ def test_calls_of_threads_with_sizes_of_their_own(T):
     assert not errors
     work(8192)
     assert not errors and T.device_error() == 0
+
+
+# ------------------------------------------------------------------------------------------------ autograd
+def test_gradients_are_refused_and_writes_are_seen(T):
+    """There is no backward pass: a tensor that requires gradients is refused where they would be recorded, and autograd
+    notices that a call wrote a tensor that it had saved."""
+    rng = np.random.default_rng(25)
+    c = _cache(T, rng, 4, 2, 64, 16)
+    slots = _dev([16, 17], torch.int64)
+    x, lens, table = torch.randn((2, 2, 64), device="cuda"), _dev([1, 1], torch.int32), _dev([[1], [2]], torch.int32)
+    q, k, v, g, beta, S = _rule_inputs(rng, 2, 2, 4, 64, 32, F32, 1)
+    rule = dict(q=q, k=k, v=v, g=g, beta=beta, state=S)
+    calls = [lambda y: T.kv8_append(c, y, x, slots), lambda y: T.kv8_append(c, x, y, slots), lambda y: T.kv8_attention(c, y, table, lens),
+             lambda y: T.kv8_attention(c, x, table, lens, out=y)]
+    for call in calls:
+        with pytest.raises(T.TsbError, match="no backward pass"):
+            call(x.clone().requires_grad_())
+        with torch.no_grad():
+            call(x.clone().requires_grad_())
+        call(x.clone().requires_grad_().detach())
+    for name in rule:
+        with pytest.raises(T.TsbError, match="no backward pass"):
+            T.gated_delta(**dict(rule, **{name: rule[name].clone().requires_grad_()}))
+    with torch.no_grad():
+        T.gated_delta(**dict(rule, q=q.clone().requires_grad_()))
+
+    def changed(t, call):
+        before = t._version
+        call()
+        return t._version > before
+    append = lambda: T.kv8_append(c, x, x, slots)                     # noqa: E731
+    assert all(changed(t, append) for t in (c.k, c.v, c.k_scale, c.v_scale))
+    out = torch.empty_like(x)
+    assert changed(out, lambda: T.kv8_attention(c, x, table, lens, out=out))
+    assert not changed(c.k, lambda: T.kv8_attention(c, x, table, lens)) and not changed(x, append)
+    after, o = torch.empty_like(S), torch.empty_like(v)
+    assert changed(S, lambda: T.gated_delta(**rule)) and changed(o, lambda: T.gated_delta(**rule, out=o))
+    assert changed(after, lambda: T.gated_delta(**rule, state_out=after)) and not changed(S, lambda: T.gated_delta(**rule, state_out=after))
+    free, n = _dev([0, 1, 2, 3], torch.int32), _dev([4], torch.int32)
+    tables = lambda: T.block_tables(lens, _dev([1, 1], torch.int32), table, free, n, 16, 2)  # noqa: E731
+    assert changed(table, tables) and changed(free, tables) and not changed(lens, tables)
+    w = torch.ones_like(S, requires_grad=True)
+    loss = (w * S).sum()                                               # saves S
+    T.gated_delta(**rule)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():                                       # tensors without versions
+        T.gated_delta(**dict(rule, state=S.clone(), out=torch.empty_like(v)))
+        T.kv8_append(T.KV8Cache(2, 2, 64), x, x, slots)
+    assert T.device_error() == 0

@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -102,6 +103,17 @@ void own_memory(const at::Tensor& t, const char* what) {
         span += (t.size(order[i]) - 1) * t.stride(order[i]);
     }
 }
+// The operators have no backward pass: a tensor that asks for gradients would get outputs without them.
+void no_grad(std::initializer_list<const at::Tensor*> tensors, const char* what) {
+    if (!c10::GradMode::is_enabled()) return;
+    for (const at::Tensor* t : tensors)
+        if (t->defined() && t->requires_grad())
+            refuse(std::string(what) + ": a tensor requires gradients, and there is no backward pass: call it under torch.no_grad() or detach the tensor");
+}
+// A tensor that the call writes: what autograd saved of it before is out of date.
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 c10::Device cuda_of(const at::Tensor& t, const char* what) {
     if (!t.is_cuda()) bad(t, what, "a tensor on a CUDA device");
     return t.device();
@@ -163,6 +175,7 @@ PyObject* block_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const c10::cuda::CUDAGuard guard(dev);
         at::Tensor after = at::empty({R}, lens.options()), cu = at::empty({R + 1}, lens.options()), left = at::empty({1}, lens.options()),
                    slots = at::empty({cap}, lens.options().dtype(at::kLong));
+        written(table), written(stack);
         status(tsb_block_tables((const int32_t*) ptr(lens), (const int32_t*) ptr(add), (const uint8_t*) ptr(done), (int) R,
                                 (int32_t*) ptr(table), R > 1 ? table.stride(0) : width, (int) width, (int32_t*) ptr(stack), (int) blocks,
                                 (const int32_t*) ptr(n_free), bs, (int32_t*) ptr(after), (int32_t*) ptr(cu), (int64_t*) ptr(slots), cap,
@@ -182,6 +195,7 @@ PyObject* block_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
 struct Pools {
     tsb_kv8 c;
     c10::Device dev;
+    const at::Tensor &k, &v, &ks, &vs;
 };
 Pools pools(PyObject* o) {
     if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) refuse("KV8Cache: (k, v, k_scale, v_scale)");
@@ -200,7 +214,7 @@ Pools pools(PyObject* o) {
     need(k.size(0) <= INT32_MAX && k.size(1) <= INT32_MAX, "KV8Cache: sizes");
     return Pools{tsb_kv8{sizeof(tsb_kv8), (int32_t) k.size(0), (int32_t) k.size(2), (int32_t) k.size(1), (int32_t) k.size(3),
                          (int8_t*) ptr(k), (int8_t*) ptr(v), (float*) ptr(ks), (float*) ptr(vs)},
-                 dev};
+                 dev, k, v, ks, vs};
 }
 
 // (cache, k, v, slots)
@@ -215,7 +229,10 @@ PyObject* kv8_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         rows(k, T, p.c.n_kv_heads, p.c.head_dim, k.scalar_type(), p.dev, "kv8_append: k");
         rows(v, T, p.c.n_kv_heads, p.c.head_dim, k.scalar_type(), p.dev, "kv8_append: v");
         flat(slots, at::kLong, T, p.dev, "kv8_append: slots");
+        no_grad({&k, &v, &p.ks, &p.vs}, "kv8_append");
         const c10::cuda::CUDAGuard guard(p.dev);
+        if (T)
+            for (const at::Tensor* t : {&p.k, &p.v, &p.ks, &p.vs}) written(*t);
         status(tsb_kv8_append(&p.c, ptr(k), ptr(v), e, k.stride(0), k.stride(1), v.stride(0), v.stride(1), (const int64_t*) ptr(slots), T,
                               stream_of(p.dev)),
                "kv8_append");
@@ -232,6 +249,7 @@ PyObject* kv8_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
         on(slots, at::kLong, 1, p.dev, "kv8_read: slots");
         const int64_t T = slots.size(0);
         flat(slots, at::kLong, T, p.dev, "kv8_read: slots");
+        no_grad({&p.ks, &p.vs}, "kv8_read");
         const int e = int32(a[2], "kv8_read: dtype");
         const at::ScalarType type = e == 0 ? at::kFloat : e == 1 ? at::kHalf : at::kBFloat16;
         const c10::cuda::CUDAGuard guard(p.dev);
@@ -266,8 +284,9 @@ PyObject* kv8_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         flat(lens, at::kInt, R, p.dev, "kv8_attention: lens");
         if (cu.defined()) flat(cu, at::kInt, R + 1, p.dev, "kv8_attention: cu_q");
         need(R <= INT32_MAX && heads <= INT32_MAX && width <= INT32_MAX, "kv8_attention: sizes");
+        no_grad({&q, &out, &p.ks, &p.vs}, "kv8_attention");
         const c10::cuda::CUDAGuard guard(p.dev);
-        if (out.defined()) rows(out, T, heads, p.c.head_dim, q.scalar_type(), p.dev, "kv8_attention: out"), own_memory(out, "kv8_attention: out");
+        if (out.defined()) rows(out, T, heads, p.c.head_dim, q.scalar_type(), p.dev, "kv8_attention: out"), own_memory(out, "kv8_attention: out"), written(out);
         else out = at::empty({T, heads, p.c.head_dim}, q.options());
         d.n_req = (int32_t) R, d.q_heads = (int32_t) heads, d.table_width = (int32_t) width;
         if (a[5] != Py_None) d.max_q = int32(a[5], "kv8_attention: max_q");
@@ -320,6 +339,7 @@ PyObject* gated_delta(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const char *s0 = (const char*) ptr(state), *s1 = (const char*) ptr(after);
         if (s0 != s1 && s0 < s1 + after.nbytes() && s1 < s0 + state.nbytes())
             bad(after, "gated_delta: state_out", "state itself or memory of its own");
+        no_grad({&q, &k, &v, &g, &beta, &state, &after, &out}, "gated_delta");
         const int64_t max_len = a[7] == Py_None ? T : integer(a[7]), slots = state.size(0);
         int64_t B;
         if (cu.defined()) {
@@ -335,7 +355,7 @@ PyObject* gated_delta(PyObject*, PyObject* const* a, Py_ssize_t n) {
         else need(slots >= B, "gated_delta: a state for every sequence");
         need(max_len >= 0 && max_len <= INT32_MAX && B <= INT32_MAX && slots <= INT32_MAX && hv <= INT32_MAX && dv <= INT32_MAX, "gated_delta: sizes");
         const c10::cuda::CUDAGuard guard(dev);
-        if (out.defined()) rows(out, T, hv, dv, type, dev, "gated_delta: out"), own_memory(out, "gated_delta: out");
+        if (out.defined()) rows(out, T, hv, dv, type, dev, "gated_delta: out"), own_memory(out, "gated_delta: out"), written(out);
         else out = at::empty({T, hv, dv}, q.options());
         d.n_seq = (int32_t) B, d.max_len = (int32_t) max_len, d.k_heads = (int32_t) hk, d.v_heads = (int32_t) hv;
         d.dim_k = (int32_t) dk, d.dim_v = (int32_t) dv, d.n_states = (int32_t) slots;
@@ -346,6 +366,7 @@ PyObject* gated_delta(PyObject*, PyObject* const* a, Py_ssize_t n) {
         d.eps = (float) number(a[12]);
         d.n_tok = T, d.q_tok = q.stride(0), d.q_head = q.stride(1), d.k_tok = k.stride(0), d.k_head = k.stride(1);
         d.v_tok = v.stride(0), d.v_head = v.stride(1), d.o_tok = out.stride(0), d.o_head = out.stride(1), d.gb_tok = g.stride(0);
+        written(after);
         const uint64_t size = tsb_gated_delta_workspace_bytes(&d);
         const at::Tensor ws = bytes(size, dev);
         status(tsb_gated_delta(&d, ptr(q), ptr(k), ptr(v), (const float*) ptr(g), (const float*) ptr(beta), (const float*) ptr(state),

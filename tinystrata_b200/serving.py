@@ -7,8 +7,9 @@ and both feed a ``MoELayer`` / ``PrefillLayer``.
 
 Every call is asynchronous on ``stream`` (default: the current stream of the tensors' device), takes its workspace and new
 outputs from torch's allocator for that stream, and raises ``TsbError`` where an argument is refused.  Tensors may be
-strided; the innermost dimension must be contiguous.  The calls go through ``_serving.so`` (csrc/tsb_pyserving.cpp), built
-beside libtsb_moe.so; without it they raise.
+strided; the innermost dimension must be contiguous.  There is no backward pass: with autograd on, a tensor that requires
+gradients is refused, and tensors that a call writes count as changed in place.  The calls go through ``_serving.so``
+(csrc/tsb_pyserving.cpp), built beside libtsb_moe.so; without it they raise.
 """
 from __future__ import annotations
 
