@@ -299,3 +299,16 @@ def test_gradients_are_refused_and_writes_are_seen(T):
         T.gated_delta(**dict(rule, state=S.clone(), out=torch.empty_like(v)))
         T.kv8_append(T.KV8Cache(2, 2, 64), x, x, slots)
     assert T.device_error() == 0
+
+
+def test_delta_one_token_has_no_row_stride(T):
+    """The strides of a single row are arbitrary: g from a product of its own beside beta from a wider one."""
+    rng = np.random.default_rng(35)
+    q, k, v, g, beta, S = _rule_inputs(rng, 1, 2, 4, 64, 32, F32, 1)
+    ro, rs = R.gated_delta(q, k, v, g, beta, S, [0, 1])
+    wide = torch.zeros((1, 9), device="cuda")
+    wide[:, 2:6] = beta
+    for row in (wide[:, 2:6], beta.as_strided((1, 4), (77, 1)), beta.as_strided((1, 4), (0, 1))):
+        o, s = T.gated_delta(q, k, v, g, row, S, state_out=torch.empty_like(S))
+        _near(o, ro, 1e-5)
+        _near(s, rs, 1e-5)

@@ -328,7 +328,7 @@ PyObject* gated_delta(PyObject*, PyObject* const* a, Py_ssize_t n) {
         rows(v, T, hv, dv, type, dev, "gated_delta: v");
         for (const at::Tensor* t : {&g, &beta}) {
             on(*t, at::kFloat, 2, dev, "gated_delta: g, beta");
-            if (t->size(0) != T || t->size(1) != hv || (hv > 1 && t->stride(1) != 1) || t->stride(0) != g.stride(0))
+            if (t->size(0) != T || t->size(1) != hv || (hv > 1 && t->stride(1) != 1) || (T > 1 && t->stride(0) != g.stride(0)))
                 bad(*t, "gated_delta: g, beta", "[tokens, v_heads], rows contiguous and of one stride,");
         }
         on(state, at::kFloat, 4, dev, "gated_delta: state");

@@ -133,8 +133,8 @@ def gated_delta(q, k, v, g, beta, state, cu_seqlens=None, max_len: int | None = 
                 scale: float | None = None, qk_norm: bool = False, eps: float = 1e-6, out=None, stream=None):
     """The gated delta rule over packed sequences (tsb_gated_delta).
 
-    q, k [T, k_heads, dim_k], v [T, v_heads, dim_v] of one type; g (log decays) and beta fp32 [T, v_heads]; state fp32
-    [n_states, v_heads, dim_k, dim_v].  cu_seqlens int32 [B + 1] bounds the sequences (None: T / max_len sequences of
+    q, k [T, k_heads, dim_k], v [T, v_heads, dim_v] of one type; g (log decays) and beta fp32 [T, v_heads], their rows of
+    one stride; state fp32 [n_states, v_heads, dim_k, dim_v].  cu_seqlens int32 [B + 1] bounds the sequences (None: T / max_len sequences of
     max_len tokens; max_len default T, else at least the longest one).  state_idx int32 [B] names the sequences' states
     (None: in order; negative: from zeros, not kept).  What they ask beyond max_len, T or the states is left out and
     recorded in ``device_error()``; rows of no sequence stay as out had them (a new one: undefined).  The states after the step go to state_out (default: in place; else
