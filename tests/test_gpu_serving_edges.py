@@ -312,3 +312,28 @@ def test_delta_one_token_has_no_row_stride(T):
         o, s = T.gated_delta(q, k, v, g, row, S, state_out=torch.empty_like(S))
         _near(o, ro, 1e-5)
         _near(s, rs, 1e-5)
+
+
+# ------------------------------------------------------------------------------------------------ waits
+def test_short_wait_limits(T):
+    """Under the shortest bound a wait may give up, which the device error word says; the context and the next calls are as
+    before."""
+    rng = np.random.default_rng(26)
+    c = _cache(T, rng, 300, 4, 128, 16)
+    lens = [2000, 900]
+    table, dl = _tables(rng, lens, 16, 300), _dev(lens, torch.int32)
+    q = torch.randn((1600, 16, 128), device="cuda").to(BF16)
+    x = _rule_inputs(rng, 600, 8, 8, 128, 128, BF16, 1)
+    run = lambda: [T.kv8_attention(c, q, table, dl, max_q=800), *T.gated_delta(*x, state_out=torch.empty_like(x[-1]))]  # noqa: E731
+    good = run()
+    assert T.device_error() == 0
+    T.set_wait_limit_ns(100_000)
+    try:
+        for _ in range(5):
+            short = run()
+            if T.device_error() == 0:
+                assert all(torch.equal(a, b) for a, b in zip(short, good))
+    finally:
+        T.set_wait_limit_ns(2_000_000_000)
+    assert all(torch.equal(a, b) for a, b in zip(run(), good))
+    assert T.device_error() == 0

@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_attn_prompt(const __grid_
     constexpr int N = P::kN, NG = P::kGroups, CH = D / 16;       // CH: 16-code chunks of a token
     extern __shared__ __align__(1024) uint8_t prompt_smem[];
     uint8_t* smem = prompt_smem + ((1024 - (smem_u32(prompt_smem) & 1023)) & 1023);
-    __shared__ uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], s_free[2], p_full[2], pv_done[2];
+    __shared__ uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], s_free[2], p_full[2], pv_done[2], drained;
     __shared__ uint32_t tbase;
     __shared__ float rowf[128], meet[2][2][128], sums[2][128];
     __shared__ float heads[4][3][NG];                             // key scales, value scales, whether the block is in the cache
@@ -119,6 +119,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_attn_prompt(const __grid_
             mbar_init(&k_full[i], 8), mbar_init(&k_empty[i], 1), mbar_init(&v_full[i], 8), mbar_init(&v_empty[i], 1);
             mbar_init(&s_full[i], 2), mbar_init(&s_free[i], 8), mbar_init(&p_full[i], 8), mbar_init(&pv_done[i], 1);
         }
+        mbar_init(&drained, 1);
         fence_mbar_init();
     }
     if (warp == kMmaWarp) {
@@ -414,7 +415,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_attn_prompt(const __grid_
             return true;
         };
         bool ok = n > 0 && scores(0);
-        int done = 0;
         for (int j = 0; j < n && ok; ++j) {
             const int b = j & 1;
             if (j + 1 < n && !(ok = scores(j + 1))) break;
@@ -431,10 +431,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_attn_prompt(const __grid_
             }
             umma_commit(&v_empty[b]);
             umma_commit(&pv_done[b]);
-            ++done;
         }
-        // products in flight end before the CTA's memory goes
-        if (!ok && done > 0) mbar_wait_bounded(&pv_done[(done - 1) & 1], ((done - 1) >> 1) & 1, p.err, kSitePrompt);
+        if (!ok && n > 0) {                                       // every product so far, the scores ahead among them
+            umma_commit(&drained);
+            mbar_drain(&drained, 0, p.err, kSitePrompt);
+        }
     }
     __syncwarp();
     tc_fence_before();

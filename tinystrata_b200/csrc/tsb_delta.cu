@@ -846,6 +846,15 @@ __global__ void __launch_bounds__(256, kScanCtas<DK, W>) k_delta_scan(const Delt
     const int br = (lane & 7) + (lane >> 4) * 8, tr = (lane & 7) + ((lane >> 3) & 1) * 8;
     const uint32_t row_x = (((lane >> 3) & 1) ^ (br & 7)) << 4, col_x = ((lane >> 4) ^ (tr & 7)) << 4;
     bool ok = true;
+    // after a wait that gave up: the copies of chunks c .. to - 1 land before the CTA's memory goes
+    auto land = [&](int c, int to) {
+        for (; c < min(to, chunks); ++c) mbar_drain(&full[c & 1], (c >> 1) & 1, p.err, kSiteDelta);
+    };
+    auto wait_tiles = [&](int c) {
+        if (!ok) return;
+        ok = mbar_wait_bounded(&full[c & 1], (c >> 1) & 1, p.err, kSiteDelta);
+        if (!ok && fetches) land(c, c + 2);
+    };
     // a chunk's tiles are read by all 8 warps; then those of the chunk after the next take their place
     auto release = [&](int c) {
         __syncwarp();
@@ -853,6 +862,7 @@ __global__ void __launch_bounds__(256, kScanCtas<DK, W>) k_delta_scan(const Delt
         if (fetches && c + 2 < chunks && ok) {
             ok = mbar_wait_bounded(&empty[c & 1], (c >> 1) & 1, p.err, kSiteDelta);
             if (ok) fetch(c + 2);
+            else land(c + 1, c + 2);
         }
     };
     // Z^T: tokens' states' part of the outputs
@@ -930,10 +940,6 @@ __global__ void __launch_bounds__(256, kScanCtas<DK, W>) k_delta_scan(const Delt
             }
         }
     };
-    auto in_flight = [&]() {                    // after a wait that gave up: copies land before the CTA's memory goes
-        for (int i = 0; i < 2; ++i)
-            for (int ph = 0; ph < 2; ++ph) mbar_wait_bounded(&full[i], ph, p.err, kSiteDelta);
-    };
     if constexpr (W == 2) {
         if (writer) {                           // meets the same barriers as the warps that carry the states, and knows their scales
             auto meet_state = [&]() {
@@ -960,7 +966,7 @@ __global__ void __launch_bounds__(256, kScanCtas<DK, W>) k_delta_scan(const Delt
             for (int c = 0; c < chunks; ++c) {
                 const int i = c & 1;
                 if (c + 1 < chunks) load_values(c + 1);
-                if (ok) ok = mbar_wait_bounded(&full[i], (c >> 1) & 1, p.err, kSiteDelta);
+                wait_tiles(c);
                 const uint32_t kt = smem_u32(sm + i * T::kStage), mt = kt + T::kHead;
                 const float* vec = (const float*) (sm + i * T::kStage + T::kHead + (2 + T::PP) * T::kSq);
                 float Z[NP * 2][4];
@@ -1011,7 +1017,6 @@ __global__ void __launch_bounds__(256, kScanCtas<DK, W>) k_delta_scan(const Delt
                 release(c);
                 if (c + 1 < chunks) meet_state();
             }
-            if (!ok) in_flight();
             return;
         }
     }
@@ -1020,7 +1025,7 @@ __global__ void __launch_bounds__(256, kScanCtas<DK, W>) k_delta_scan(const Delt
     for (int c = 0; c < chunks; ++c) {
         const int i = c & 1;
         // after a wait that gave up the loop runs on over whatever the tiles hold, so that every barrier is met
-        if (ok) ok = mbar_wait_bounded(&full[i], (c >> 1) & 1, p.err, kSiteDelta);
+        wait_tiles(c);
         const uint32_t kt = smem_u32(sm + i * T::kStage), mt = kt + T::kHead;
         const uint32_t kr = kt + br * RB, mr = mt + br * SB, kc = kt + tr * RB;
         const float* vec = (const float*) (sm + i * T::kStage + T::kHead + (2 + T::PP) * T::kSq);
@@ -1226,11 +1231,7 @@ __global__ void __launch_bounds__(256, kScanCtas<DK, W>) k_delta_scan(const Delt
             share_state();
         }
     }
-    if (!ok) {
-        in_flight();
-        return;
-    }
-    if (st >= 0 && in) {
+    if (ok && st >= 0 && in) {
 #pragma unroll
         for (int i = 0; i < NK; ++i)
 #pragma unroll

@@ -193,9 +193,9 @@ __device__ __forceinline__ uint64_t globaltimer() {
 static __device__ unsigned long long g_wait_ns = 2000000000ull;
 __device__ __forceinline__ uint64_t wait_limit_ns() { return g_wait_ns; }
 
-__device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, unsigned* err, unsigned site) {
+__device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, unsigned* err, unsigned site, uint64_t least = 0) {
     if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = globaltimer(), lim = wait_limit_ns();
+    const uint64_t t0 = globaltimer(), lim = max(wait_limit_ns(), least);
     for (uint32_t i = 1;; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((i & 255u) == 0 && globaltimer() - t0 > lim) {
@@ -203,6 +203,12 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
             return false;
         }
     }
+}
+
+// Before a kernel that gave up returns: the end of its own copies or products in flight, whose memory goes with it.  They take
+// microseconds, but not less than the bound that the caller may have set, so this wait has a bound of its own.
+__device__ __forceinline__ bool mbar_drain(uint64_t* bar, uint32_t parity, unsigned* err, unsigned site) {
+    return mbar_wait_bounded(bar, parity, err, site, 2000000000ull);
 }
 
 // The same with test_wait polls (never suspended): for a wait on the critical path whose phase usually completes within
