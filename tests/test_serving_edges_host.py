@@ -53,3 +53,34 @@ def test_no_device_is_an_error():
         assert tables(n=n) == CUDA, n
         assert "block_tables" in T.last_error()
     assert attend() == CUDA and attend(n_req=4000, cu=A, n_tok=8000) == CUDA
+
+
+def test_native_module_is_rebuilt_for_another_torch(monkeypatch, tmp_path):
+    """_serving.so is bound to the torch it was built against: another version makes it stale, the same one does not."""
+    from tinystrata_b200 import build
+    ext, runs = tmp_path / "_serving.so", []
+
+    class Done:
+        returncode = 0
+
+    def run(cmd, **kw):
+        runs.append(cmd)
+        ext.write_bytes(b"")
+        return Done
+
+    monkeypatch.setattr(build, "EXT", str(ext))
+    monkeypatch.setattr(build, "EXT_FOR", str(tmp_path / "_serving.torch"))
+    monkeypatch.setattr(build.subprocess, "run", run)
+    build.build_ext()
+    build.build_ext()
+    assert len(runs) == 1
+    monkeypatch.setattr(torch, "__version__", "99.0")
+    build.build_ext()
+    build.build_ext()
+    assert len(runs) == 2
+    Done.returncode, Done.stderr = 1, "no"
+    monkeypatch.setattr(torch, "__version__", "99.1")
+    for _ in range(2):                              # a build that failed is not taken for one
+        with pytest.raises(RuntimeError):
+            build.build_ext()
+    assert len(runs) == 4

@@ -13,6 +13,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtsb_moe.so")
 EXT = os.path.join(HERE, "_serving.so")          # the CPython module over the library (tinystrata_b200/serving.py)
+EXT_FOR = os.path.join(HERE, "_build", "_serving.torch")   # the torch that it was built against
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 SOURCES = ["tsb_moe.cu", "tsb_decode.cu", "tsb_decode_act.cu", "tsb_ep.cu", "tsb_staged.cu", "tsb_cache.cu",
            "tsb_delta.cu", "tsb_gguf.cpp"]
@@ -68,16 +69,22 @@ def build_ext(verbose: bool = False, force: bool = False) -> str:
     """The native Python module of the serving-step operators: C++ against torch's headers and the library beside it."""
     import sysconfig
 
-    src = os.path.join(CSRC, "tsb_pyserving.cpp")
-    if not (force or _stale(EXT, [src, os.path.join(HERE, "..", "include", "tsb_moe.h")])):
-        return EXT
     import torch
+
+    src = os.path.join(CSRC, "tsb_pyserving.cpp")
+    abi = int(torch.compiled_with_cxx11_abi())
+    tag, known = f"torch {torch.__version__}, C++11 ABI {abi}\n", ""
+    if os.path.exists(EXT_FOR):
+        with open(EXT_FOR) as f:
+            known = f.read()
+    if not (force or known != tag or _stale(EXT, [src, os.path.join(HERE, "..", "include", "tsb_moe.h")])):
+        return EXT
     root = os.path.dirname(torch.__file__)
     inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
            sysconfig.get_paths()["include"], os.path.join(os.path.dirname(NVCC), "..", "include")]
     libs = os.path.join(root, "lib")
     cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *[f"-I{i}" for i in inc], src, "-o", EXT,
+           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *[f"-I{i}" for i in inc], src, "-o", EXT,
            f"-L{HERE}", "-l:libtsb_moe.so", f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
            "-Wl,-rpath,$ORIGIN"]
     if verbose:
@@ -85,6 +92,9 @@ def build_ext(verbose: bool = False, force: bool = False) -> str:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed on tsb_pyserving.cpp:\n{r.stderr}")
+    os.makedirs(os.path.dirname(EXT_FOR), exist_ok=True)
+    with open(EXT_FOR, "w") as f:
+        f.write(tag)
     return EXT
 
 
