@@ -380,8 +380,9 @@ int tsb_block_tables(const int32_t* lens, const int32_t* n_new, const uint8_t* d
                      int32_t* n_free_out, void* stream);
 
 /* Append n_tok tokens' keys and values ([token][head][head_dim] with the strides given) at slots (as tsb_block_tables
- * writes them; one outside the cache is skipped).  Tokens of one block follow one another in `slots`, ascending.  Per
- * (block, head): scale' = max(scale, largest magnitude / 127), the scale counting as 0 when the tokens start the block;
+ * writes them; one outside the cache is skipped).  Tokens of one block stand in `slots` in their order and as far apart as in
+ * the block (skipped ones may lie between them); those between two skipped ones are a run, and runs are appended one after
+ * the other.  Per (block, head) and run: scale' = max(scale, largest magnitude / 127), the scale counting as 0 when the tokens start the block;
  * codes already there become rint(code * (scale / scale')), new ones rint(x / scale').  NaN is stored as 0, an infinity
  * as the largest bf16. */
 int tsb_kv8_append(const tsb_kv8* cache, const void* k, const void* v, int elem_type, int64_t k_tok, int64_t k_head,

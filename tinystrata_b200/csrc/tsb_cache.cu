@@ -319,8 +319,44 @@ __device__ __forceinline__ uint4 rescale_codes(uint4 w, float ratio) {
     return w;
 }
 
+// The slots of a token's neighbours, lane by lane: at[..] of token t on, before[..] back from t - 1 (the second 32 in blocks
+// of 64; -1 past the ends).
+struct Near {
+    int64_t at[2], before[2];
+};
+__device__ __forceinline__ Near near_slots(const AppendParams& p, int64_t t, int lane) {
+    Near n;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int64_t up = t + i * 32 + lane, down = t - 1 - i * 32 - lane;
+        const bool use = i == 0 || p.c.bs > 32;
+        n.at[i] = use && up < p.n_tok ? p.slots[up] : -1;
+        n.before[i] = use && down >= 0 ? p.slots[down] : -1;
+    }
+    return n;
+}
+// Whether an earlier token of the call is in the block of the token at s: in its place before it, skipped ones between or not.
+__device__ __forceinline__ bool follows(const Near& n, int64_t s, int off, int lane) {
+    return __any_sync(0xffffffffu, (lane < off && n.before[0] == s - 1 - lane) || (lane + 32 < off && n.before[1] == s - 33 - lane));
+}
+// The call's tokens in that block from it on: bit i, the token i places after it, at s + i.
+__device__ __forceinline__ uint64_t block_tokens(const Near& n, int64_t s, int room, int lane) {
+    const unsigned lo = __ballot_sync(0xffffffffu, lane < room && n.at[0] == s + lane);
+    const unsigned hi = __ballot_sync(0xffffffffu, lane + 32 < room && n.at[1] == s + 32 + lane);
+    return (uint64_t) hi << 32 | lo;
+}
+// The first run of those tokens, taken out of them: its first place and its length.
+__device__ __forceinline__ int next_run(uint64_t& tokens, int& len) {
+    const int skip = __ffsll((long long) tokens) - 1;
+    const uint64_t rest = tokens >> skip;
+    len = rest == ~0ull ? 64 : __ffsll((long long) ~rest) - 1;
+    tokens = skip + len < 64 ? tokens >> (skip + len) << (skip + len) : 0;
+    return skip;
+}
+
 // Warp (keys or values, head, token), for decode steps, where nearly every token is a run of its own.  A run is the tokens
-// of one call that follow one another within one cache block; its first token is the leader, and its warp takes the run:
+// of one call that follow one another within one cache block; the block's first token is the leader, and its warp takes the
+// block's runs, of which there are several only around skipped tokens, one after the other:
 // the largest magnitude over it, the block's new scale max(old, largest / 127) (old: none when the run starts the block), the block's earlier codes
 // brought to it when it grew, and the run's codes.  One warp owns the (block, head), so no value is written twice and
 // nothing is atomic.  Divisions are IEEE: the same codes on any device.  Bound by the chain of loads: slots, rows, scale
@@ -336,42 +372,40 @@ __global__ void __launch_bounds__(128) k_kv8_append(const AppendParams p) {
     if (t >= p.n_tok) return;
     const void* src = is_v ? p.v : p.k;
     const int64_t row = is_v ? p.v_tok : p.k_tok, col = (is_v ? p.v_head : p.k_head) * h;
-    const int64_t s = p.slots[t], before = t ? p.slots[t - 1] : -2;
-    if (s < 0 || s >= cap || ((s & (bs - 1)) && before == s - 1)) return;
-    const int64_t blk = s >> p.c.shift;
-    const int off = (int) (s & (bs - 1));
-    int n = 0;                                       // tokens of the run
-    for (int b0 = 0; b0 < bs - off; b0 += 32) {
-        const int i = b0 + lane;
-        const bool in = i < bs - off && t + i < p.n_tok && p.slots[t + i] == s + i;
-        const unsigned b = __ballot_sync(0xffffffffu, in);
-        n += b == 0xffffffffu ? 32 : __ffs(~b) - 1;
-        if (b != 0xffffffffu) break;
-    }
+    const Near near = near_slots(p, t, lane);
+    const int64_t s = __shfl_sync(0xffffffffu, near.at[0], 0), blk = s >> p.c.shift;
+    const int at = (int) (s & (bs - 1));
+    if (s < 0 || s >= cap || follows(near, s, at, lane)) return;
     int8_t* codes = (is_v ? p.c.v : p.c.k) + ((blk * p.c.H + h) << p.c.shift) * D;
     float* sp = (is_v ? p.c.vs : p.c.ks) + blk * p.c.H + h;
-    const float was = off > 0 ? *sp : 0.0f;
-    float peak = 0.0f;
+    for (uint64_t todo = block_tokens(near, s, bs - at, lane); todo;) {
+        int n;
+        const int skip = next_run(todo, n), off = at + skip;
+        const int64_t t0 = t + skip;
+        const float was = off > 0 ? *sp : 0.0f;
+        float peak = 0.0f;
 #pragma unroll 4
-    for (int e = lane; e < n * DV; e += 32) {
-        float x[8];
-        load8(x, src, (t + (e >> dvs)) * row + col + (e & (DV - 1)) * 8, p.type, p.wide);
-        peak = fmaxf(peak, peak_value(x));
-    }
-    peak = warp_max(peak);
-    const float now = fmaxf(was, peak / kCodeMax), inv = 1.0f / now;
-    __syncwarp();
-    if (lane == 0) *sp = now;
-    if (off > 0 && now != was) {
-        const float ratio = was / now;
-        for (int e = lane; e < off * D / 16; e += 32) ((uint4*) codes)[e] = rescale_codes(((const uint4*) codes)[e], ratio);
-    }
+        for (int e = lane; e < n * DV; e += 32) {
+            float x[8];
+            load8(x, src, (t0 + (e >> dvs)) * row + col + (e & (DV - 1)) * 8, p.type, p.wide);
+            peak = fmaxf(peak, peak_value(x));
+        }
+        peak = warp_max(peak);
+        const float now = fmaxf(was, peak / kCodeMax), inv = 1.0f / now;
+        __syncwarp();
+        if (lane == 0) *sp = now;
+        if (off > 0 && now != was) {
+            const float ratio = was / now;
+            for (int e = lane; e < off * D / 16; e += 32) ((uint4*) codes)[e] = rescale_codes(((const uint4*) codes)[e], ratio);
+        }
 #pragma unroll 4
-    for (int e = lane; e < n * DV; e += 32) {
-        float x[8];
-        load8(x, src, (t + (e >> dvs)) * row + col + (e & (DV - 1)) * 8, p.type, p.wide);
-        peak_value(x);
-        *(uint2*) (codes + (int64_t) off * D + (int64_t) e * 8) = encode8(x, now, inv);
+        for (int e = lane; e < n * DV; e += 32) {
+            float x[8];
+            load8(x, src, (t0 + (e >> dvs)) * row + col + (e & (DV - 1)) * 8, p.type, p.wide);
+            peak_value(x);
+            *(uint2*) (codes + (int64_t) off * D + (int64_t) e * 8) = encode8(x, now, inv);
+        }
+        __syncwarp();                                    // the next run reads the scale and the codes
     }
 }
 
@@ -398,62 +432,62 @@ __global__ void __launch_bounds__(128) k_kv8_append_runs(const AppendParams p) {
             leads = s >= 0 && s < cap && ((s & (bs - 1)) == 0 || before != s - 1);
         }
         for (unsigned todo = __ballot_sync(0xffffffffu, leads); todo; todo &= todo - 1) {
-            const int64_t t = base_t + __ffs(todo) - 1, s = p.slots[t], blk = s >> p.c.shift;
-            const int off = (int) (s & (bs - 1));
-            int n = 0;
-            for (int b0 = 0; b0 < bs - off; b0 += 32) {
-                const int i = b0 + lane;
-                const bool in = i < bs - off && t + i < p.n_tok && p.slots[t + i] == s + i;
-                const unsigned b = __ballot_sync(0xffffffffu, in);
-                n += b == 0xffffffffu ? 32 : __ffs(~b) - 1;
-                if (b != 0xffffffffu) break;
-            }
+            const int64_t first = base_t + __ffs(todo) - 1;
+            const Near near = near_slots(p, first, lane);
+            const int64_t s = __shfl_sync(0xffffffffu, near.at[0], 0), blk = s >> p.c.shift;
+            const int place = (int) (s & (bs - 1));
+            if (follows(near, s, place, lane)) continue;
             int8_t* codes = (is_v ? p.c.v : p.c.k) + ((blk * p.c.H + h) << p.c.shift) * D;
             float* sp = (is_v ? p.c.vs : p.c.ks) + blk * p.c.H + h;
-            const float was = off > 0 ? *sp : 0.0f;
-            constexpr int HOLD = 8;
-            float x[HOLD][8], peak = 0.0f;
-            auto at = [&](int e) { return (t + (e >> dvs)) * row + col + (e & (DV - 1)) * 8; };
+            for (uint64_t runs = block_tokens(near, s, bs - place, lane); runs;) {
+                int n;
+                const int skip = next_run(runs, n), off = place + skip;
+                const int64_t t = first + skip;
+                const float was = off > 0 ? *sp : 0.0f;
+                constexpr int HOLD = 8;
+                float x[HOLD][8], peak = 0.0f;
+                auto at = [&](int e) { return (t + (e >> dvs)) * row + col + (e & (DV - 1)) * 8; };
 #pragma unroll
-            for (int i = 0; i < HOLD; ++i) {
-                const int e = i * 128 + tid;
-                if (e < n * DV) load8(x[i], src, at(e), p.type, p.wide);
-            }
+                for (int i = 0; i < HOLD; ++i) {
+                    const int e = i * 128 + tid;
+                    if (e < n * DV) load8(x[i], src, at(e), p.type, p.wide);
+                }
 #pragma unroll
-            for (int i = 0; i < HOLD; ++i) {
-                if (i * 128 + tid >= n * DV) break;
-                peak = fmaxf(peak, peak_value(x[i]));
-            }
-            for (int e = HOLD * 128 + tid; e < n * DV; e += 128) {         // longer runs: the rest is read twice
-                float y[8];
-                load8(y, src, at(e), p.type, p.wide);
-                peak = fmaxf(peak, peak_value(y));
-            }
-            peak = warp_max(peak);
-            if (lane == 0) peaks[warp] = peak;
-            __syncthreads();                                               // also: every thread has read the old scale
-            peak = fmaxf(fmaxf(peaks[0], peaks[1]), fmaxf(peaks[2], peaks[3]));
-            const float now = fmaxf(was, peak / kCodeMax), inv = 1.0f / now;
-            if (tid == 0) *sp = now;
-            if (off > 0 && now != was) {
-                const float ratio = was / now;
-                for (int e = tid; e < off * D / 16; e += 128) ((uint4*) codes)[e] = rescale_codes(((const uint4*) codes)[e], ratio);
-            }
-            auto put = [&](int e, const float (&y)[8]) {
-                *(uint2*) (codes + (int64_t) off * D + (int64_t) e * 8) = encode8(y, now, inv);
-            };
+                for (int i = 0; i < HOLD; ++i) {
+                    if (i * 128 + tid >= n * DV) break;
+                    peak = fmaxf(peak, peak_value(x[i]));
+                }
+                for (int e = HOLD * 128 + tid; e < n * DV; e += 128) {         // longer runs: the rest is read twice
+                    float y[8];
+                    load8(y, src, at(e), p.type, p.wide);
+                    peak = fmaxf(peak, peak_value(y));
+                }
+                peak = warp_max(peak);
+                if (lane == 0) peaks[warp] = peak;
+                __syncthreads();                                               // also: every thread has read the old scale
+                peak = fmaxf(fmaxf(peaks[0], peaks[1]), fmaxf(peaks[2], peaks[3]));
+                const float now = fmaxf(was, peak / kCodeMax), inv = 1.0f / now;
+                if (tid == 0) *sp = now;
+                if (off > 0 && now != was) {
+                    const float ratio = was / now;
+                    for (int e = tid; e < off * D / 16; e += 128) ((uint4*) codes)[e] = rescale_codes(((const uint4*) codes)[e], ratio);
+                }
+                auto put = [&](int e, const float (&y)[8]) {
+                    *(uint2*) (codes + (int64_t) off * D + (int64_t) e * 8) = encode8(y, now, inv);
+                };
 #pragma unroll
-            for (int i = 0; i < HOLD; ++i) {
-                const int e = i * 128 + tid;
-                if (e < n * DV) put(e, x[i]);
+                for (int i = 0; i < HOLD; ++i) {
+                    const int e = i * 128 + tid;
+                    if (e < n * DV) put(e, x[i]);
+                }
+                for (int e = HOLD * 128 + tid; e < n * DV; e += 128) {
+                    float y[8];
+                    load8(y, src, at(e), p.type, p.wide);
+                    peak_value(y);
+                    put(e, y);
+                }
+                __syncthreads();                                               // peaks are read
             }
-            for (int e = HOLD * 128 + tid; e < n * DV; e += 128) {
-                float y[8];
-                load8(y, src, at(e), p.type, p.wide);
-                peak_value(y);
-                put(e, y);
-            }
-            __syncthreads();                                               // peaks are read
         }
     }
 }

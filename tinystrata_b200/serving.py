@@ -95,7 +95,7 @@ class KV8Cache:
 
 def kv8_append(cache: KV8Cache, k, v, slots, stream=None) -> None:
     """Keys and values [T, n_kv_heads, head_dim] into the cache at slots int64 [T] (tsb_kv8_append); -1 skips a token.
-    Tokens of one block follow one another in slots, ascending."""
+    Tokens of one block follow one another in slots, ascending, with skipped ones in their places."""
     if stream is not None:
         with _on(stream):
             return kv8_append(cache, k, v, slots)
