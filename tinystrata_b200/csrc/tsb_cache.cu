@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(128) k_kv8_append(const AppendParams p) {
 // The same for prompts: CTA (chunk of block_size tokens, head, keys or values), the run's values in registers between the
 // two passes (up to 64 a thread; a warp's two passes over 16 KB went to memory twice: 82 us for 16,024 tokens of 8 heads).
 // Now 64 us for those in fp32, 164 MB: the codes' arithmetic and the memory about equally.
-__global__ void __launch_bounds__(128) k_kv8_append_runs(const AppendParams p) {
+__global__ void __launch_bounds__(128, 5) k_kv8_append_runs(const AppendParams p) {
     __shared__ float peaks[4];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int bs = p.c.bs, D = p.c.D, DV = D / 8, dvs = D == 64 ? 3 : D == 128 ? 4 : 5;
@@ -427,16 +427,18 @@ __global__ void __launch_bounds__(128) k_kv8_append_runs(const AppendParams p) {
     for (int64_t base_t = start; base_t < end_t; base_t += 32) {          // every warp finds the leaders for itself
         const int64_t mine = base_t + lane;
         bool leads = false;
+        int64_t slot = -1;
         if (mine < end_t) {
-            const int64_t s = p.slots[mine], before = mine ? p.slots[mine - 1] : -2;
-            leads = s >= 0 && s < cap && ((s & (bs - 1)) == 0 || before != s - 1);
+            slot = p.slots[mine];
+            const int64_t before = mine ? p.slots[mine - 1] : -2;
+            leads = slot >= 0 && slot < cap && ((slot & (bs - 1)) == 0 || before != slot - 1);
         }
         for (unsigned todo = __ballot_sync(0xffffffffu, leads); todo; todo &= todo - 1) {
             const int64_t first = base_t + __ffs(todo) - 1;
-            const Near near = near_slots(p, first, lane);
-            const int64_t s = __shfl_sync(0xffffffffu, near.at[0], 0), blk = s >> p.c.shift;
+            const int64_t s = __shfl_sync(0xffffffffu, slot, __ffs(todo) - 1), blk = s >> p.c.shift;
             const int place = (int) (s & (bs - 1));
-            if (follows(near, s, place, lane)) continue;
+            const Near near = near_slots(p, first, lane);
+            if (place > 1 && follows(near, s, place, lane)) continue;
             int8_t* codes = (is_v ? p.c.v : p.c.k) + ((blk * p.c.H + h) << p.c.shift) * D;
             float* sp = (is_v ? p.c.vs : p.c.ks) + blk * p.c.H + h;
             for (uint64_t runs = block_tokens(near, s, bs - place, lane); runs;) {
