@@ -136,7 +136,7 @@ __device__ __forceinline__ int last_le(const int* a, int n, int64_t v) {
 // which block a token's position lands in follows from the prefix sums alone, so no CTA reads what another writes.
 // The stack of free blocks is free_list[0 .. n_free) with the blocks given back on top of it; the k-th block taken is
 // the k-th from the top.  What bounds it is the launch and the dependent loads (lengths, then list or table): at 8
-// requests nothing else is left (5.2 us), at 1000 requests and 33,000 tokens the slots' 8 bytes a token are 0.3 MB (8.7 us).
+// requests nothing else is left (5.6 us), at 1000 requests and 33,000 tokens the slots' 8 bytes a token are 0.3 MB (9.2 us).
 __global__ void __launch_bounds__(kTabThreads) k_block_tables(const TabParams p) {
     extern __shared__ int sh[];
     const int R = p.n_req;
@@ -360,7 +360,7 @@ __device__ __forceinline__ int next_run(uint64_t& tokens, int& len) {
 // the largest magnitude over it, the block's new scale max(old, largest / 127) (old: none when the run starts the block), the block's earlier codes
 // brought to it when it grew, and the run's codes.  One warp owns the (block, head), so no value is written twice and
 // nothing is atomic.  Divisions are IEEE: the same codes on any device.  Bound by the chain of loads: slots, rows, scale
-// (48 tokens of 2 heads of 256: 3.2 us).
+// (48 tokens of 2 heads of 256: 3.1 us).
 __global__ void __launch_bounds__(128) k_kv8_append(const AppendParams p) {
     const int lane = threadIdx.x & 31;
     const int bs = p.c.bs, D = p.c.D, DV = D / 8, dvs = D == 64 ? 3 : D == 128 ? 4 : 5;
@@ -411,7 +411,8 @@ __global__ void __launch_bounds__(128) k_kv8_append(const AppendParams p) {
 
 // The same for prompts: CTA (chunk of block_size tokens, head, keys or values), the run's values in registers between the
 // two passes (up to 64 a thread; a warp's two passes over 16 KB went to memory twice: 82 us for 16,024 tokens of 8 heads).
-// Now 64 us for those in fp32, 164 MB: the codes' arithmetic and the memory about equally.
+// Now 61 us for those in fp32, 164 MB, 2.7 TB/s: the latency of load, maximum and codes one after the other at 20 warps a SM
+// (issue slots 46% active; a warp waits 2.1 cycles an instruction for its own results, 2.0 for memory, 1.8 for instructions).
 __global__ void __launch_bounds__(128, 5) k_kv8_append_runs(const AppendParams p) {
     __shared__ float peaks[4];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -495,8 +496,9 @@ __global__ void __launch_bounds__(128, 5) k_kv8_append_runs(const AppendParams p
 }
 
 // CTA (share of the tokens, head, keys or values): four codes a thread and step, so that a warp's stores of 16 (8) bytes a
-// lane are consecutive, eight steps in flight.  A slot outside the cache reads as zeros.  Bound by the bytes: 16,024 tokens of
-// 8 heads of 128 to fp32 (164 MB) take 45 us.
+// lane are consecutive, eight steps in flight.  A slot outside the cache reads as zeros.  Bound by latency, slot after slot to
+// codes and scale: 16,024 tokens of 8 heads of 128 to fp32 (164 MB) take 45 us, 3.7 TB/s, with the issue slots 42% active and
+// a warp waiting 11.6 cycles an instruction for memory.
 constexpr int kReadSteps = 8;
 __global__ void __launch_bounds__(256) k_kv8_read(const Cache c, const int64_t* __restrict__ slots, int64_t n_tok,
                                                   void* k, void* v, int type) {
@@ -1017,8 +1019,9 @@ constexpr int kSplitCtas = NB == 1 ? (D == 256 ? 3 : D == 128 ? 4 : 5) : (D == 2
 // end of each segment.  A segment inside one range is finished there; one cut by a range's end leaves its rows, maxima
 // and sums for k_attn_join.  So a lone request of 131,072 tokens and 64 requests of uneven lengths fill the GPU alike.
 // Bound by memory with one query a request (32 requests of 8192 tokens, heads of 128: 5.7 TB/s; 2 of 131,072, heads of 256,
-// fp32: 58 us, 4.6 TB/s), by the issue of the score planes' products with more (64 of up to 8192 with up to 3: 139 us,
-// 3.9 TB/s).
+// fp32: 59 us, 4.6 TB/s), by latency with more (64 of up to 8192 with up to 3: 139 us, 4.0 TB/s): the two groups' rows leave
+// 12 warps a SM (168 registers), issue slots are 53% active, and the chain of products, maxima and weights is what a warp
+// waits for (1.6 cycles an instruction), not a pipe.
 template <int D, int SP, int NB>
 __global__ void __launch_bounds__(kAttnWarps * 32, kSplitCtas<D, NB>) k_attn_split(const __grid_constant__ AttnParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
@@ -1284,7 +1287,9 @@ __global__ void __launch_bounds__(256) k_attn_check(const __grid_constant__ Attn
 
 // Many rows of fp32 queries: one warp per tile of 32 rows (head_dim 256: 16), every step of the tile by the same warp, which turns a
 // step's codes into operands once for all of them; the four warps of a CTA take neighbouring tiles of a head, so they share
-// the codes through the caches.  Bound by the products, three planes a score: 843 queries of 8 heads over 2000 keys 209 us.
+// the codes through the caches.  Bound by the latency of a step's products and weights at 8 warps a SM (255 registers; issue
+// slots 41% active): 843 queries of 32 heads over 8, 2000 keys, heads of 128, 271 us, 80 TFLOP/s; of 8 heads over one, which are
+// 53 CTAs, 209.
 template <int D>
 constexpr int kTileGroups = D == 256 ? 2 : 4;
 template <int D>
@@ -1489,7 +1494,11 @@ int tsb_kv8_append(const tsb_kv8* cache, const void* k, const void* v, int elem_
     AppendParams p{cache_of(cache), k, v, elem_type, k_tok, k_head, v_tok, v_head, slots, n_tok, false};
     p.wide = !((uintptr_t) k % 16 || (uintptr_t) v % 16 || (k_tok * es) % 16 || (k_head * es) % 16 || (v_tok * es) % 16 ||
                (v_head * es) % 16);
-    // few tokens are decode steps, a run each: a warp a token; many are prompts: a CTA a block's worth
+    // Few tokens are taken for decode steps, a run each: a warp a token; many for prompts: a CTA a block's worth.  What decides
+    // is the length of the runs, which only the device knows.  Measured, a warp a token against a CTA a block's worth (us,
+    // 8 heads of 128, bf16, blocks of 16): requests of one token, 256 of them 4 against 29, 1024 10 against 59, 4000 31 against
+    // 175; one prompt of 64 tokens 10 against 4, of 1000 12 against 8, of 4000 24 against 20.  So up to 1024 tokens a wrong guess
+    // costs 2 to 6 us and is made for prompts; above, it costs most in steps of thousands of requests.
     const bool few = n_tok <= 1024;
     const int64_t ctas = few ? (n_tok + 3) / 4 : (n_tok + cache->block_size - 1) / cache->block_size;
     if (ctas > 0x7fffffffll / 2 / cache->n_kv_heads) return cfail(TSB_ERR_UNSUPPORTED, "kv8_append: too many tokens");

@@ -111,8 +111,9 @@ __device__ __forceinline__ float4 ld_state(const float* p) {     // volatile: is
 // CTA (32 value columns, value head, sequence): the state's slice in registers, thread (row group of 32, 4 columns):
 // dim_k / 32 rows of four columns.  One reduction over dim_k a token: S^T k and S^T q of the decayed state together,
 // o = scale (S^T q + (q . k) u), so the second product needs no second pass.  Single tokens are bound by the state's
-// bytes, read and written once: 128 of them with 32 heads of 128 x 128 (540 MB) take 100 us, 5.4 TB/s (119 while every thread
-// summed the warps' parts for its columns, which one warp does now); 5 and 6 CTAs a SM measured 105 and 111 against 103.
+// bytes, read and written once: 128 of them with 32 heads of 128 x 128 (540 MB) take 100 to 106 us a pass on different boards, 5.1
+// to 5.4 TB/s (119 while every thread summed the warps' parts for its columns, which one warp does now); 5 and 6 CTAs a SM
+// measured 105 and 111 against 103.
 template <int DK>
 __global__ void __launch_bounds__(256, 4) k_delta_step(const DeltaParams p) {
     constexpr int RPT = DK / 32;
@@ -381,7 +382,9 @@ __device__ __forceinline__ void merge_blocks(float* X, float* tmp, int tid) {
 // workspace; K K^T and Q K^T on the tensor cores (warp w: rows 16 w); then for each value head of the key head the
 // decays, A, P and M.  (1 + A)^-1 in fp32 from its 8 x 8 diagonal blocks (forward substitution, a thread a column) by
 // three joins of neighbouring blocks: exact arithmetic on the triangle, where powers of A would cancel, with every
-// thread at work (one thread a column over all 64 rows is 2000 dependent steps: 240 us for 8192 tokens, 32 heads; now 148).
+// thread at work (one thread a column over all 64 rows is 2000 dependent steps: 240 us for 8192 tokens, 32 heads; now 149).
+// Bound by latency: a value head's dozen steps lie between barriers, issue slots are 29% active, and a warp waits 3.7 cycles an
+// instruction for shared and 3.6 for global memory (16-bit forms spill some 140 bytes at 128 registers).
 template <int E, int DK>
 __global__ void __launch_bounds__(128, E == E_F32 ? 2 : 4) k_delta_prepare(const DeltaParams p) {
     using T = Tiles<E, DK>;
@@ -691,11 +694,11 @@ struct RowScale {
 // Z and O, which no later chunk waits for, from the same exchanges, and bring V.  What bounds it: a sequence's chunks
 // follow one another, and a unit's 400 products of 16 x 8 x 16 a chunk (bf16, dim_k 128) at 8 cycles each.  One sequence
 // of 32 heads has 256 units, so W 2 puts them on 128 SMs with every scheduler at work; with more sequences W 1 does the
-// same work without exchanges.  8192 tokens of 32 heads, bf16: 329 us, a chunk in 4670 cycles, of which the products before the
-// next chunk take 2140 and the exchanges 1590.
+// same work without exchanges.  8192 tokens of 32 heads, bf16: 314 us, a chunk in some 4460 cycles.  (Stamped when it took 329:
+// 4670 cycles, of which the products before the next chunk took 2140 and the exchanges 1590.)
 // W 2 at dim_k 128 fills a SM's shared memory with one CTA, and is told so: with the 128 registers that two would leave it
-// 8192 tokens take 496 us a pass, with 227 461.  The other forms are left to the compiler (W 1 told the same: 257 against
-// 240 for 16 sequences of 256).
+// 8192 tokens take 504 us a pass, with 231 466.  The other forms are left to the compiler (W 1 told the same: 304 against
+// 286 for 4 sequences of 1000 in fp32).
 template <int DK, int W>
 constexpr int kScanCtas = W == 2 && DK == 128 ? 1 : 0;
 template <int E, int DK, int W>
@@ -1241,7 +1244,10 @@ __global__ void __launch_bounds__(256, kScanCtas<DK, W>) k_delta_scan(const Delt
 }
 
 // ------------------------------------------------------------------------------------------------ host
-constexpr int kStepTokens = 16;      // sequences up to this many tokens run the recurrence
+// Sequences of up to this many tokens run the recurrence.  Measured, the recurrence against chunks (us, 32 heads of 128, bf16): one
+// sequence of 16 tokens 17 against 27, of 24 25 against 27, of 32 32 against 28; 16 of 8 tokens 47 against 71, of 16 86 against 77;
+// 64 of 8 177 against 230, of 16 331 against 248.  (The chunks' error is larger: states 3e-7 against 1e-7 of 64 bits.)
+constexpr int kStepTokens = 16;
 
 int delta_check(const tsb_delta_desc* d) {
     if (!d || d->struct_size != sizeof(tsb_delta_desc)) return dfail(TSB_ERR_ARG, "gated_delta: struct_size");
@@ -1287,8 +1293,8 @@ int launch_chunks(const DeltaParams& p, cudaStream_t st) {
     if (int rc = dcuda("gated_delta: chunks")) return rc;
     // W 1 does less in all and W 2 a chunk sooner, so W 1 where the chunks of all sequences outweigh the longest one's, and where its
     // eight units a CTA have 16 columns each.  Measured with 32 heads of 128 (us a pass, W 1 against W 2): one sequence of 8192
-    // tokens 1324 against 477, 8 ragged ones up to 1024 208 against 174 (fp32); 4 of 1000 245 against 257 (fp32 268 against 334), 16
-    // of 256 259 against 276, 64 of 64 281 against 425; 16 of 256 with 6 heads 73 against 78; with heads of 64 143 against 128.
+    // tokens 1221 against 466, 8 ragged ones up to 1024 234 against 170 (fp32); 4 of 1000 226 against 249 (fp32 286 against 323), 16
+    // of 256 248 against 272, 64 of 64 290 against 431; 16 of 256 with 6 heads 78 against 78; with heads of 64 143 against 128.
     const int64_t longest = (p.max_len + kChunk - 1) / kChunk;
     const bool many = p.dv > 64 && (int64_t) p.max_chunks * p.hv * 5 >= longest * sm_count() * 3;
     return many ? launch_scan<E, DK, 1>(p, st) : launch_scan<E, DK, 2>(p, st);
