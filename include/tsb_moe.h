@@ -407,8 +407,8 @@ uint64_t tsb_kv8_attention_workspace_bytes(const tsb_kv8* cache, const tsb_kv8_a
  * of q are cu_q[r] .. cu_q[r + 1] (null: max_q rows each), row i of n sits at position lens[r] - n + i and sees the keys
  * up to its position.  Query head h reads key / value head h / (q_heads / n_kv_heads).  A row without keys is zero.
  * Scores, maxima, sums and outputs are accumulated in fp32; out has q's type.  A block id outside the cache hides its
- * keys.  A request with more than max_q rows, or rows past n_tok, is cut there and recorded in the device error word; rows
- * of no request are not written.  At most 4096 requests of at most 2^31 - 1025 tokens (table_width * block_size).
+ * keys.  A request with more than max_q rows, rows past n_tok or a length past its row of the table is cut there and recorded
+ * in the device error word; rows of no request are not written.  At most 4096 requests of at most 2^31 - 1025 tokens (table_width * block_size).
  * Workspace 16-byte aligned, its size from the query above (0 when none is needed). */
 int tsb_kv8_attention(const tsb_kv8* cache, const tsb_kv8_attn* d, const void* q, const int32_t* table, const int32_t* lens,
                       const int32_t* cu_q, void* out, void* workspace, uint64_t ws_bytes, void* stream);

@@ -135,6 +135,21 @@ def test_attention_every_row_by_default(T, dtype, queries, lens, H, G):
     assert T.device_error() == 0
 
 
+@pytest.mark.parametrize("n,H,dtype", [(1, 2, BF16), (230, 4, BF16), (230, 8, F32)])
+def test_attention_says_when_a_length_passes_its_table(T, n, H, dtype):
+    """A length beyond the table's columns is cut, with its queries at its end, which the device error word says."""
+    rng = np.random.default_rng(27)
+    c = _cache(T, rng, 64, H, 64, 16)
+    table = _tables(rng, [400, 300], 16, 64)
+    q = torch.randn((2 * n, 4 * H, 64), device="cuda").to(dtype)
+    for cu in (None, _dev([0, n, 2 * n], torch.int32)):
+        kw = dict(cu_q=cu, max_q=n)
+        got = T.kv8_attention(c, q, table, _dev([401, 300], torch.int32), **kw)
+        assert T.device_error() == 0xC0000003
+        assert torch.equal(got, T.kv8_attention(c, q, table, _dev([400, 300], torch.int32), **kw))
+        assert T.device_error() == 0
+
+
 # ------------------------------------------------------------------------------------------------ gated delta rule
 # k heads, v heads, dim_k, dim_v, sequences: two warps a unit (64 and 128 wide), and one (many sequences)
 RULE_FORMS = [(1, 2, 64, 64, 1), (2, 4, 128, 128, 1), (4, 8, 128, 128, 30)]

@@ -580,9 +580,11 @@ __device__ __forceinline__ Req attn_req(const AttnParams& p, int r) {
     }
     return q;
 }
-constexpr unsigned kSiteRows = 0xC0000002u;   // the error word when a request has more than max_q rows, or rows past n_tok
+constexpr unsigned kSiteRows = 0xC0000002u;   // the error word when a request has more than max_q rows, or rows past n_tok,
+constexpr unsigned kSiteKeys = 0xC0000003u;   // and when its length passes its row of the table
 __device__ __forceinline__ void check_request(const AttnParams& p, int r) {
     if (p.cu && (int64_t) p.cu[r + 1] > min((int64_t) max(p.cu[r], 0) + p.max_q, p.n_tok)) report_error(p.err, kSiteRows);
+    if ((int64_t) p.lens[r] > (int64_t) p.width * p.c.bs) report_error(p.err, kSiteKeys);
 }
 // The first key of row i's window (below zero when it holds all of them).  A row without keys counts as position -1: the
 // difference stays in 32 bits for every window.
@@ -1280,8 +1282,9 @@ __global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ AttnP
 }
 
 // check_request for k_attn_tiles, whose registers are so full that the same lines inside it cost 4 to 7% (843 queries over 2000
-// keys: 281 to 290 us against 271 without and 274 with this launch).
+// keys: 281 to 290 us against 271 without and 276 with this launch).
 __global__ void __launch_bounds__(256) k_attn_check(const __grid_constant__ AttnParams p) {
+    asm volatile("griddepcontrol.launch_dependents;");
     for (int r = threadIdx.x; r < p.n_req; r += 256) check_request(p, r);
 }
 
@@ -1437,8 +1440,20 @@ int launch_attn(const AttnParams& p, const AttnPlan& a, int rows, cudaStream_t s
         static std::atomic<bool> granted[kMaxDev];
         const int sm = kAttnWarps * (kTileGroups<D> * 3 * (D / 32) * 256 + 128 + Ring<D>::kBytes);
         if (int rc = allow_smem(k_attn_tiles<D>, granted, sm, "kv8_attention: shared memory")) return rc;
-        if (p.cu) k_attn_check<<<1, 256, 0, st>>>(p);
-        k_attn_tiles<D><<<dim3((unsigned) ((p.tiles + kAttnWarps - 1) / kAttnWarps), p.c.H, p.n_req), kAttnWarps * 32, sm, st>>>(p);
+        k_attn_check<<<1, 256, 0, st>>>(p);
+        if (int rc = ccuda("kv8_attention: check")) return rc;
+        // the tiles come up beside the check, on which nothing of theirs depends
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned) ((p.tiles + kAttnWarps - 1) / kAttnWarps), p.c.H, p.n_req);
+        cfg.blockDim = dim3(kAttnWarps * 32);
+        cfg.dynamicSmemBytes = sm;
+        cfg.stream = st;
+        cudaLaunchAttribute at{};
+        at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+        cudaLaunchKernelEx(&cfg, k_attn_tiles<D>, p);
     }
     return ccuda("kv8_attention");
 }

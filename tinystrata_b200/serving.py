@@ -119,9 +119,10 @@ def kv8_attention(cache: KV8Cache, q, table, lens, cu_q=None, max_q: int | None 
     q [T, q_heads, head_dim]; table int32 [R, W] and lens int32 [R] as ``block_tables`` leaves them (the queries' own keys
     appended; requests may share rows of the table, as samples of one prompt do: ``table.expand``); cu_q int32 [R + 1]
     bounds of the requests' rows in q (None: max_q rows each); max_q at least the most rows of a request (default 1, with
-    cu_q all rows of q; a close bound is faster, and a request with more rows is cut and recorded in ``device_error()``);
-    window 0 or the number of last keys a query sees; scale default head_dim ** -0.5.  Returns out, of q's shape and type
-    (its elements share no memory); rows of no request stay as out had them (a new one: undefined)."""
+    cu_q all rows of q; a close bound is faster; a request with more rows, or longer than its row of the table, is cut and
+    recorded in ``device_error()``); window 0 or the number of last keys a query sees; scale default head_dim ** -0.5.
+    Returns out, of q's shape and type (its elements share no memory); rows of no request stay as out had them (a new one:
+    undefined)."""
     if stream is not None:
         with _on(stream):
             return kv8_attention(cache, q, table, lens, cu_q, max_q, window, scale, out)
