@@ -156,6 +156,36 @@ def test_attention_queries_that_are_not_finite(T, n, H, dtype):
     assert T.device_error() == 0
 
 
+@pytest.mark.parametrize("n,H,dtype", FORMS)
+def test_attention_forms_repeat_and_capture(T, n, H, dtype):
+    """The same bits twice, on another stream, and replayed from a graph after lengths and queries changed."""
+    rng = np.random.default_rng(47)
+    lens, bs = [700, 400], 16
+    NB = sum(R.blocks_of(x, bs) for x in lens)
+    c = _cache(T, rng, NB, H, 64, bs)
+    table, dl, cu = _tables(rng, lens, bs, NB), _dev(lens, torch.int32), _dev([0, n, 2 * n], torch.int32)
+    q = torch.randn((2 * n, 4 * H, 64), device="cuda").to(dtype)
+    kw = dict(table=table, lens=dl, cu_q=cu, max_q=n)
+    good = T.kv8_attention(c, q, **kw)
+    assert torch.equal(T.kv8_attention(c, q, **kw), good)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    other = T.kv8_attention(c, q, **kw, stream=side)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(other, good)
+    out = torch.empty_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        T.kv8_attention(c, q, **kw, out=out)
+    graph.replay()
+    assert torch.equal(out, good)
+    dl.copy_(_dev([523, 399], torch.int32))
+    q.mul_(0.5)
+    graph.replay()
+    assert torch.equal(out, T.kv8_attention(c, q, **kw)) and not torch.equal(out, good)
+    assert T.device_error() == 0
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("n,H", [(1, 2), (3, 2), (230, 4)])
 def test_attention_fp16_outputs_keep_their_bits(T, n, H, D):
